@@ -46,6 +46,12 @@ class LayeredConfig(C.Structure):
                 ("loop_stop", _u32), ("loop_times", _u32)]
 
 
+class PagedKvDesc(C.Structure):
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("page_table", _p), ("seq_lens", _p), ("k_page_stride", _sz), ("k_slot_stride", _sz),
+                ("k_head_stride", _sz), ("v_page_stride", _sz), ("v_slot_stride", _sz), ("v_head_stride", _sz), ("type", _i32),
+                ("n_pages", _u32), ("page_size", _u32), ("n_kv_heads", _u32), ("head_dim", _u32), ("n_seqs", _u32), ("max_pages", _u32)]
+
+
 # name -> (restype, argtypes); every symbol include/cera_cuda.h declares.
 SIGNATURES = {
     "cera_cuda_last_error": (C.c_char_p, []),
@@ -70,6 +76,12 @@ SIGNATURES = {
     "cera_cuda_decode_attention": (_i32, [_p, _p, _p, _i32, _sz, _sz, _sz, _sz, _f, _p, _p, _sz, _p]),
     "cera_cuda_prefill_attention": (_i32, [_p, _p, _p, _i32, _sz, _sz, _sz, _sz, _sz, _f, _p, _p]),
     "cera_cuda_decode_attention_noalloc": (_i32, [_p, _p, _p, _i32, _sz, _sz, _sz, _sz, _f, _p, _p]),
+    "cera_cuda_paged_append": (_i32, [_p, _p, _p, _i32, _p, _sz, _p, _p, _sz, _p, _p]),
+    "cera_cuda_paged_decode_attention_workspace_bytes": (_sz, [_p, _sz, _i32]),
+    "cera_cuda_paged_decode_attention": (_i32, [_p, _p, _i32, _sz, _f, _u32, _u32, _p, _sz, _p, _p, _sz, _p]),
+    "cera_cuda_paged_prefill_attention_workspace_bytes": (_sz, [_p, _sz, _sz]),
+    "cera_cuda_paged_prefill_attention": (_i32, [_p, _p, _i32, _sz, _p, _sz, _f, _u32, _u32, _p, _p, _sz, _p]),
+    "cera_cuda_paged_evict": (_i32, [_p, _p, _p, _sz, _sz, _u32, _u32, _p, _p, _sz, _p, _p, _p]),
     "cera_cuda_synth_normal": (_i32, [_p, _sz, _u64, _u64, _f, _p]),
     "cera_cuda_quantize_weights": (_i32, [_i32, _p, _sz, _p, _p]),
     "cera_cuda_model_create": (_i32, [C.POINTER(Config), C.POINTER(_p)]),

@@ -1,0 +1,33 @@
+// A paged key/value cache as kernels see it, and the launches of what reads and writes it.
+#pragma once
+
+#include "common.cuh"
+
+namespace cera {
+
+// Strides in bytes.  A quotient by the page size is (n * page_mul) >> page_shift, exact for n below 2^31.
+struct PagedView {
+    uint8_t *k, *v;
+    const int32_t *table, *lens;
+    size_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    uint32_t page_mul, page_shift, page_size, n_pages, hk, dim, n_seqs, max_pages;
+};
+
+// What a query in slot p sees of the slots: j <= p, and with a window j < sink or j > p - window.
+struct PagedMask {
+    uint32_t window, sink;
+};
+
+int32_t launch_paged_append(const PagedView &kv, int type, const void *k, const void *v, int src_type, const int32_t *starts, size_t n, float *weights,
+                            int32_t *positions, size_t track_stride, const int32_t *token_pos, cudaStream_t st);
+size_t paged_decode_workspace(const PagedView &kv, size_t n_heads, bool weights);
+int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, float scale, PagedMask mask, float *weights,
+                            size_t weights_stride, void *out, void *ws, cudaStream_t st);
+size_t paged_prefill_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);
+int32_t launch_paged_prefill(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
+                             PagedMask mask, void *out, void *ws, cudaStream_t st);
+int32_t launch_paged_evict(const PagedView &kv, int type, const float *weights, const int32_t *positions, size_t track_stride, size_t budget, uint32_t n_sink,
+                           uint32_t n_recent, float *weights_out, int32_t *positions_out, size_t out_stride, int32_t *kept, int32_t *lens_out,
+                           cudaStream_t st);
+
+}  // namespace cera

@@ -1,0 +1,204 @@
+"""A paged key/value cache of several sequences, and the operators that read and write it: storing new rows, attention of one token per
+sequence and of portions of prompts, with a sliding window and first tokens that stay visible, and eviction by accumulated attention
+weight.  The reference keeps one sequence in contiguous rows (cera/src/kv_cache.rs:201-221) and has no counterpart.
+
+Like the other operator calls these take torch CUDA tensors as device memory, launch on torch's current stream and never wait."""
+import ctypes as C
+
+import torch
+
+from . import ops
+from ._lib import PagedKvDesc, check, lib
+from .types import BF16, F16, F32
+
+_TYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _current():
+    return ops._device() if ops._device else torch.cuda.current_device()
+
+
+def _take(t, what, dtype, shape, device):
+    """t as a contiguous tensor of that type and shape (None: any extent) on the cache's device."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise TypeError(f"{what}: expected a tensor on {device}, where the cache is")
+    if t.dtype != dtype or not t.is_contiguous():
+        raise TypeError(f"{what}: expected a contiguous {dtype} tensor, got {t.dtype}")
+    if t.dim() != len(shape) or any(a is not None and a != b for a, b in zip(shape, t.shape)):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class PagedKv:
+    """The tensors of a cache, which stay the caller's: k_pages and v_pages [n_pages, page_size, n_kv_heads, head_dim] of float32, float16 or
+    bfloat16 in any strides of whole 16 bytes (head_dim contiguous; keys and values may be interleaved views of one tensor),
+    page_table int32 [n_seqs, max_pages] and seq_lens int32 [n_seqs].  Slot j of sequence s is row j % page_size of page
+    page_table[s, j // page_size]; an entry outside [0, n_pages) is a page that is not there, whose slots are not seen.  The calls read the
+    table and the lengths when they run, so both may be changed in place between calls and under a captured graph."""
+
+    def __init__(self, k_pages, v_pages, page_table, seq_lens):
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("seq_lens", seq_lens)):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda):
+                raise TypeError(f"{name}: expected a CUDA tensor: this path has no CPU fallback")
+            if t.device != k_pages.device:
+                raise ValueError(f"{name} is on {t.device}, k_pages on {k_pages.device}")
+        if k_pages.dtype not in _TYPE or v_pages.dtype != k_pages.dtype:
+            raise TypeError(f"pages must both be float32, float16 or bfloat16, got {k_pages.dtype} and {v_pages.dtype}")
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+            raise ValueError(f"pages are [n_pages, page_size, n_kv_heads, head_dim], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if t.stride(3) != 1 or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+                raise ValueError(f"{name}: head_dim must be contiguous and no row may stand for several, got strides {t.stride()}")
+        if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0]:
+            raise ValueError(f"page_table [n_seqs, max_pages] and seq_lens [n_seqs] do not go together: {tuple(page_table.shape)}, {tuple(seq_lens.shape)}")
+        for name, t in (("page_table", page_table), ("seq_lens", seq_lens)):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise TypeError(f"{name}: expected a contiguous int32 tensor, got {t.dtype}")
+        self.k_pages, self.v_pages, self.page_table, self.seq_lens = k_pages, v_pages, page_table, seq_lens
+        n_pages, page_size, n_kv_heads, head_dim = k_pages.shape
+        self.n_seqs, self.n_kv_heads, self.head_dim, self.page_size = seq_lens.shape[0], n_kv_heads, head_dim, page_size
+        self.capacity = page_table.shape[1] * page_size  # slots of a sequence
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        # the stride of an extent of one is no stride
+        ks, vs = ([st if n > 1 else 0 for n, st in zip(t.shape, t.stride())] for t in (k_pages, v_pages))
+        self._desc = PagedKvDesc(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                                 _TYPE[k_pages.dtype], n_pages, page_size, n_kv_heads, head_dim, self.n_seqs, page_table.shape[1])
+        self._ref = C.byref(self._desc)
+        self._workspace = {}
+
+    def _here(self):
+        if self.device.index != _current():
+            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{_current()}: make the cache's device current")
+        return self._ref
+
+    def _rows(self, t, what, shape):
+        """Rows of the cache's type or float32."""
+        if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
+            return _take(t, what, torch.float32, shape, self.device)
+        return _take(t, what, self.dtype, shape, self.device)
+
+    def _track(self, t, what, dtype):
+        p = _take(t, what, dtype, (self.n_seqs, self.n_kv_heads, None), self.device)
+        if t.shape[2] < self.capacity:
+            raise ValueError(f"{what}: {t.shape[2]} slots, a sequence has {self.capacity}")
+        return p
+
+    def _scratch(self, workspace, key, ask):
+        need = self._workspace.get(key)
+        if need is None:
+            need = ask()
+            if need == 0:
+                raise ValueError(ops._lib.last_error())
+            if len(self._workspace) > 64:  # a program whose calls differ in size
+                self._workspace.clear()
+            self._workspace[key] = need
+        if workspace is None:
+            return torch.empty(need, dtype=torch.uint8, device=self.device)
+        _take(workspace, "workspace", torch.uint8, (None,), self.device)
+        if workspace.shape[0] < need:
+            raise ValueError(f"workspace: {workspace.shape[0]} bytes, {need} needed")
+        return workspace
+
+
+def _visible(window, n_sink):
+    if not (0 <= window < 2**32 and 0 <= n_sink < 2**32):
+        raise ValueError(f"window {window} and n_sink {n_sink}: counts of slots")
+
+
+def _starts(cache, starts):
+    return None if starts is None else _take(starts, "starts", torch.int32, (cache.n_seqs + 1,), cache.device)
+
+
+def paged_append(cache, k, v, starts=None, weights=None, positions=None, token_positions=None):
+    """Stores new tokens' keys and values, [n_tokens, n_kv_heads, head_dim] of the cache's type or float32 (rounded), in slots that
+    seq_lens already counts: sequence s's tokens [starts[s], starts[s + 1]) - int32 [n_seqs + 1]; None: one token each - go to its last slots.
+    Per slot and head, [n_seqs, n_kv_heads, at least capacity]: weights (float32) becomes 0, positions (int32) the token's position out of
+    token_positions, int32 [n_tokens] (None: its slot)."""
+    ref = cache._here()
+    shape = (None, cache.n_kv_heads, cache.head_dim)
+    kp, vp = cache._rows(k, "k", shape), cache._rows(v, "v", shape)
+    n = k.shape[0]
+    if v.shape[0] != n or v.dtype != k.dtype:
+        raise ValueError(f"k and v differ: {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    wp = pp = tp = None
+    stride = 0
+    if weights is not None:
+        wp, stride = cache._track(weights, "weights", torch.float32), weights.shape[2]
+    if positions is not None:
+        pp, stride = cache._track(positions, "positions", torch.int32), positions.shape[2]
+        if weights is not None and weights.shape[2] != stride:
+            raise ValueError("weights and positions differ in their slots")
+    if token_positions is not None:
+        tp = _take(token_positions, "token_positions", torch.int32, (n,), cache.device)
+    check(lib.cera_cuda_paged_append(ref, kp, vp, _TYPE[k.dtype], _starts(cache, starts), n, wp, pp, stride, tp, ops._stream()))
+
+
+def paged_decode_attention(cache, q, scale, window=0, n_sink=0, weights=None, out=None, workspace=None):
+    """Attention of every sequence's newest token, which is in its last slot: q [n_seqs, n_heads, head_dim] of the cache's type or float32;
+    the result is of q's type.  window: only that many last slots are seen, and the first n_sink (0: all).  weights, float32
+    [n_seqs, n_kv_heads, at least capacity], has the probabilities of a KV head's query heads added to their slots.  A sequence
+    without slots gives zeros.  Calls that may overlap need a workspace each; by default every call has its own."""
+    ref = cache._here()
+    qp = cache._rows(q, "q", (cache.n_seqs, None, cache.head_dim))
+    _visible(window, n_sink)
+    heads, stride, wp = q.shape[1], 0, None
+    if weights is not None:
+        wp, stride = cache._track(weights, "weights", torch.float32), weights.shape[2]
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _take(out, "out", q.dtype, q.shape, cache.device)
+    ws = cache._scratch(workspace, ("decode", heads, wp is not None),
+                        lambda: lib.cera_cuda_paged_decode_attention_workspace_bytes(ref, heads, int(wp is not None)))
+    check(lib.cera_cuda_paged_decode_attention(ref, qp, _TYPE[q.dtype], heads, scale, window, n_sink, wp, stride, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                               ops._stream()))
+    return out
+
+
+def paged_prefill_attention(cache, q, starts, scale, window=0, n_sink=0, out=None, workspace=None):
+    """Causal attention of portions of prompts: q [n_tokens, n_heads, head_dim], of which sequence s has [starts[s], starts[s + 1])
+    (int32 [n_seqs + 1], ascending from 0) in its last slots.  Types, window and n_sink as in paged_decode_attention, the window counted
+    back from each query.  Rows past starts[n_seqs] are left as they are in `out`, and undefined without one."""
+    ref = cache._here()
+    qp = cache._rows(q, "q", (None, None, cache.head_dim))
+    if starts is None:
+        raise TypeError("starts: expected an int32 tensor")
+    _visible(window, n_sink)
+    sp = _starts(cache, starts)
+    n, heads = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _take(out, "out", q.dtype, q.shape, cache.device)
+    ws = cache._scratch(workspace, ("prefill", heads, n), lambda: lib.cera_cuda_paged_prefill_attention_workspace_bytes(ref, heads, n))
+    check(lib.cera_cuda_paged_prefill_attention(ref, qp, _TYPE[q.dtype], heads, sp, n, scale, window, n_sink, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                ops._stream()))
+    return out
+
+
+def paged_evict(cache, weights, positions, budget, n_sink=0, n_recent=0, weights_out=None, positions_out=None, seq_lens_out=None):
+    """Cuts every sequence and KV head down to `budget` slots -> (kept, seq_lens).  Kept are the slots with a position below n_sink or
+    among the n_recent latest (newest position - n_recent < position), then those of the largest weight (a NaN is the smallest), ties
+    to the lower slot.  What is kept past the budget moves, pages included, into the gaps below it, so slots lose their order: attend without
+    a window afterwards.  weights (float32) and positions (int32), [n_seqs, n_kv_heads, at least capacity], follow in place or into
+    weights_out and positions_out (at least min(budget, capacity) slots).  kept, int32 [n_seqs, n_kv_heads, budget]: the slot that each slot's
+    content came from, -1 past the length; seq_lens: min(length, budget) in a new tensor or in seq_lens_out, which may be
+    cache.seq_lens.  Pages past the budget are the caller's again."""
+    ref = cache._here()
+    wp, pp = cache._track(weights, "weights", torch.float32), cache._track(positions, "positions", torch.int32)
+    shape = (cache.n_seqs, cache.n_kv_heads, None)
+    weights_out, positions_out = weights if weights_out is None else weights_out, positions if positions_out is None else positions_out
+    wo, po = _take(weights_out, "weights_out", torch.float32, shape, cache.device), _take(positions_out, "positions_out", torch.int32, shape, cache.device)
+    if weights.shape != positions.shape or weights_out.shape != positions_out.shape:
+        raise ValueError("weights and positions differ in their slots")
+    _visible(n_recent, n_sink)
+    if not n_sink + n_recent <= budget < 2**31 - 256 or budget < 1:
+        raise ValueError(f"a budget of {budget} slots for {n_sink} first and {n_recent} recent ones")
+    kept = torch.empty((cache.n_seqs, cache.n_kv_heads, budget), dtype=torch.int32, device=cache.device)
+    if seq_lens_out is None:
+        seq_lens_out = torch.empty_like(cache.seq_lens)
+    else:
+        _take(seq_lens_out, "seq_lens_out", torch.int32, (cache.n_seqs,), cache.device)
+    check(lib.cera_cuda_paged_evict(ref, wp, pp, weights.shape[2], budget, n_sink, n_recent, wo, po, weights_out.shape[2], kept.data_ptr(),
+                                    seq_lens_out.data_ptr(), ops._stream()))
+    return kept, seq_lens_out

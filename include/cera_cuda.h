@@ -207,6 +207,68 @@ CERA_API int32_t cera_cuda_decode_attention_noalloc(const float *q_dev, const vo
                                                     void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* A paged key/value cache of several sequences, and what reads and writes it. */
+/* No counterpart in the reference, whose cache is one sequence's rows.  A row  */
+/* is n_kv_heads heads of head_dim numbers of one type (F32, F16 or BF16); slot  */
+/* j of sequence s is row j % page_size of page page_table[s][j / page_size].     */
+/* Strides count elements; bases and strides are multiples of 16 bytes.  Slots    */
+/* [0, seq_lens[s]) are in use (a length outside [0, max_pages * page_size] counts */
+/* as the nearer end).  A table entry outside [0, n_pages) is a page that is not    */
+/* there: its slots are not seen, not stored to and not moved, so the pages that a   */
+/* window has left behind may be given back and their entries set to -1.  head_dim: */
+/* a multiple of 32 up to 256; n_seqs up to 4096.  Nothing here synchronises; lengths  */
+/* and the table are read on the device, so a captured graph follows them.            */
+typedef struct {
+    void *k_pages_dev, *v_pages_dev;
+    const int32_t *page_table_dev; /* [n_seqs][max_pages] */
+    const int32_t *seq_lens_dev;   /* [n_seqs] */
+    size_t k_page_stride, k_slot_stride, k_head_stride;
+    size_t v_page_stride, v_slot_stride, v_head_stride;
+    int32_t type;
+    uint32_t n_pages, page_size, n_kv_heads, head_dim, n_seqs, max_pages;
+} cera_cuda_paged_kv;
+
+/* Stores the keys and values of new tokens, whose slots the lengths already count: of sequence s tokens
+ * [starts[s], starts[s + 1]), starts_dev[n_seqs + 1] ascending from 0 (NULL: one token per sequence), go to its last slots.
+ * k_dev / v_dev are [n_tokens][n_kv_heads][head_dim] of `type`: the cache's, or F32, which is rounded.  Per slot and head
+ * (optional): weights_dev[n_seqs][n_kv_heads][track_stride] becomes 0 and positions_dev the token's position
+ * (token_positions_dev[n_tokens], NULL: its slot).  Tokens past starts[n_seqs] are not stored. */
+CERA_API int32_t cera_cuda_paged_append(const cera_cuda_paged_kv *kv, const void *k_dev, const void *v_dev, int32_t type,
+                                        const int32_t *starts_dev, size_t n_tokens, float *weights_dev,
+                                        int32_t *positions_dev, size_t track_stride, const int32_t *token_positions_dev,
+                                        void *stream);
+/* Attention of the newest token of every sequence, in slot p = seq_lens[s] - 1: q_dev and out_dev are
+ * [n_seqs][n_heads][head_dim] of q_type, the cache's type or F32; n_heads a multiple of n_kv_heads.  Slots j <= p are seen;
+ * with window != 0 those with j < n_sink or j > p - window.  A row that sees nothing is 0.  weights_dev (optional,
+ * [n_seqs][n_kv_heads][weights_stride]): the probabilities of a KV head's query heads are added to their slots.  workspace_dev
+ * holds cera_cuda_paged_decode_attention_workspace_bytes(...) bytes (0: an argument is refused) on a 16-byte boundary; calls that may overlap need one each. */
+CERA_API size_t cera_cuda_paged_decode_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads,
+                                                                int32_t with_weights);
+CERA_API int32_t cera_cuda_paged_decode_attention(const cera_cuda_paged_kv *kv, const void *q_dev, int32_t q_type,
+                                                  size_t n_heads, float scale, uint32_t window, uint32_t n_sink,
+                                                  float *weights_dev, size_t weights_stride, void *out_dev,
+                                                  void *workspace_dev, size_t workspace_bytes, void *stream);
+/* Causal attention of the newest tokens of every sequence, [starts[s], starts[s + 1]) of q_dev [n_tokens][n_heads][head_dim]
+ * in its last slots, with the same window and types.  Rows of out_dev past starts[n_seqs] stay as they are. */
+CERA_API size_t cera_cuda_paged_prefill_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads,
+                                                                 size_t n_tokens);
+CERA_API int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const void *q_dev, int32_t q_type,
+                                                   size_t n_heads, const int32_t *starts_dev, size_t n_tokens,
+                                                   float scale, uint32_t window, uint32_t n_sink, void *out_dev,
+                                                   void *workspace_dev, size_t workspace_bytes, void *stream);
+/* Cuts every sequence and KV head down to `budget` slots.  Kept are the slots whose position is below n_sink or among the n_recent
+ * latest (newest position - n_recent < position), then those of the largest weight (a NaN counts as the smallest), ties to the
+ * lower slot.  Kept slots below the budget stay; the others fill the gaps there, both in ascending order, so slots are in no order
+ * of position afterwards (attention without a window does not mind).  weights_dev / positions_dev are
+ * [n_seqs][n_kv_heads][track_stride]; the kept slots' go to weights_out_dev / positions_out_dev, [n_seqs][n_kv_heads][out_stride],
+ * which may be the same arrays.  kept_dev[n_seqs][n_kv_heads][budget]: the slot that each slot's content came from, -1 past the
+ * length.  seq_lens_out_dev[n_seqs] = min(length, budget), may be the cache's own lengths.  n_sink + n_recent <= budget. */
+CERA_API int32_t cera_cuda_paged_evict(const cera_cuda_paged_kv *kv, const float *weights_dev, const int32_t *positions_dev,
+                                       size_t track_stride, size_t budget, uint32_t n_sink, uint32_t n_recent,
+                                       float *weights_out_dev, int32_t *positions_out_dev, size_t out_stride,
+                                       int32_t *kept_dev, int32_t *seq_lens_out_dev, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Synthetic inputs for benchmarks and tests (the reference's counterpart is   */
 /* its converter, cera/src/convert/quantize.rs:254-343 quantize_tensor_data).  */
 /* out_dev[i] = sigma * IH12(seed, offset+i): twelve 16-bit uniforms from three */
