@@ -61,6 +61,8 @@ int32_t view(const char *what, const cera_cuda_paged_kv *kv, PagedView *out) {
     if ((((uintptr_t)kv->k_pages_dev | (uintptr_t)kv->v_pages_dev) & 15) || kv->k_page_stride % per || kv->k_slot_stride % per || kv->k_head_stride % per ||
         kv->v_page_stride % per || kv->v_slot_stride % per || kv->v_head_stride % per)
         return fail(CERA_CUDA_ERR_BAD_ARG, "%s: pages and strides must be multiples of 16 bytes", what);
+    if ((uint64_t)kv->n_seqs * ((uint64_t)kv->max_pages * kv->page_size / 32 + 1) > 0xffffffffu)
+        return fail(CERA_CUDA_ERR_BAD_ARG, "%s: %u sequences of %u pages of %u slots", what, kv->n_seqs, kv->max_pages, kv->page_size);
     if (((uintptr_t)kv->page_table_dev | (uintptr_t)kv->seq_lens_dev) & 3) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: table or lengths off a 4-byte boundary", what);
     uint32_t l = 0;
     while ((1ull << l) < kv->page_size) ++l;

@@ -25,32 +25,6 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const PagedView kv, con
     paged_attend_row<T, TQ>(kv, mask, s, h / (heads / kv.hk), len - behind, q + r * kv.dim, scale, out + r * kv.dim, lse ? lse + r : nullptr);
 }
 
-// One warp per (sequence, KV head, slot): adds its query heads' probabilities.
-template <typename T, typename TQ>
-__global__ void __launch_bounds__(128) paged_weights_kernel(const PagedView kv, const PagedMask mask, const TQ *__restrict__ q, uint32_t heads, float scale,
-                                                            const float *__restrict__ lse, float *weights, size_t stride) {
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, s = blockIdx.y, h = blockIdx.z, g = heads / kv.hk, len = paged_len(kv, s);
-    if (len == 0) return;
-    const uint32_t first = paged_first(mask, len - 1), sinks = min(mask.sink, first);
-    for (uint32_t x = blockIdx.x * 4 + (threadIdx.x >> 5); x < sinks + len - first; x += gridDim.x * 4) {
-        const uint32_t slot = x < sinks ? x : x - sinks + first;
-        uint32_t row;
-        const uint32_t page = paged_at(kv, s, slot, row);
-        if (page == NO_PAGE) continue;
-        const T *kr = reinterpret_cast<const T *>(kv.k + page * kv.k_page + row * kv.k_slot + h * kv.k_head);
-        float sum = 0.0f;
-        for (uint32_t i = 0; i < g; ++i) {
-            const size_t r = (size_t)s * heads + h * g + i;
-            float d = 0.0f;
-            for (uint32_t c = lane; c < kv.dim; c += 32) d = fmaf(to_f32(q[r * kv.dim + c]), to_f32(kr[c]), d);
-            sum += exp2f(warp_sum(d) * scale * PAGED_LOG2E - lse[r]);
-        }
-        if (lane == 0) weights[((size_t)s * kv.hk + h) * stride + slot] += sum;
-    }
-}
-
 }  // namespace
 
 template <typename F>
@@ -58,24 +32,6 @@ static int32_t by_types(int type, int q_type, F go) {
     if (type == CERA_TYPE_F32) return go(float(), float());
     if (type == CERA_TYPE_F16) return q_type == type ? go(__half(), __half()) : go(__half(), float());
     return q_type == type ? go(__nv_bfloat16(), __nv_bfloat16()) : go(__nv_bfloat16(), float());
-}
-
-size_t paged_decode_workspace(const PagedView &kv, size_t n_heads, bool weights) { return weights ? kv.n_seqs * n_heads * 4 + 16 : 16; }
-
-int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, float scale, PagedMask mask, float *weights,
-                            size_t weights_stride, void *out, void *ws, cudaStream_t st) {
-    return by_types(type, q_type, [&](auto cache, auto query) {
-        using T = decltype(cache);
-        using TQ = decltype(query);
-        count_launch();
-        CERA_CUDA_TRY(launch_k(paged_rows_kernel<T, TQ>, dim3((uint32_t)((kv.n_seqs * n_heads + 3) / 4)), dim3(128), 0, st, kv, mask, (const TQ *)q, (const int32_t *)nullptr,
-                               kv.n_seqs, (uint32_t)n_heads, scale, (TQ *)out, weights ? (float *)ws : nullptr));
-        if (!weights) return (int32_t)CERA_CUDA_OK;
-        count_launch();
-        return check_cuda(launch_k(paged_weights_kernel<T, TQ>, dim3(64, kv.n_seqs, kv.hk), dim3(128), 0, st, kv, mask, (const TQ *)q, (uint32_t)n_heads, scale,
-                                   (const float *)ws, weights, weights_stride),
-                          "paged decode attention weights launch");
-    });
 }
 
 size_t paged_prefill_workspace(const PagedView &, size_t, size_t) { return 16; }
