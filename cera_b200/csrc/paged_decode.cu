@@ -6,9 +6,11 @@
 // last unit are shared with others.  What a CTA knows of a shared unit (maximum, sum, weighted values) goes to the workspace, whose size
 // therefore does not depend on the lengths; paged_join_kernel adds the parts up in their order, so a call's bits do not depend on timing.
 //
-// A warp walks its own keys of each tile - 16 of 64 over a 16-bit cache, 8 of 32 over f32 - through a ring of its own in shared memory
-// (cp.async, 16 bytes a lane), with a running maximum, sum and weighted values of its own; warps meet at a unit's end only.  The maximum
-// is raised when a score has passed it by 2^8 (a vote, no exchange), to which the weights' range is fitted.
+// Two warps of a CTA load, keys and values, into a ring of tiles in shared memory: by TMA where a page holds whole groups of a warp's keys, a box of
+// slots an instruction (a copy for every row, by cp.async or in bulk, took most of what the kernel issued), row by row otherwise.  Four warps
+// compute, each on its own keys of a tile - 16 of 64 over a 16-bit cache, 8 of 32 over f32 - with a running maximum, sum and weighted values of
+// its own; they meet at a unit's end only.  The maximum is raised when a score has passed it by 2^8 (a vote, no exchange), to which the weights'
+// range is fitted.  Rows that are not seen are set to zero among the values: what lies there may be a NaN.
 //
 // 16-bit cache: mma.sync, 16 rows = eight heads twice: the upper half of each query and weight as the type has it, and what that leaves,
 // so an f32 query or weight counts with 22 bits (f16) in the same instructions; bf16's 16 bits are too few for an f32 query, whose third
@@ -19,18 +21,31 @@
 // With weights wanted the scaled scores are stored on the way (4 bytes a head and slot, beside the 2 dim that are read for it), and
 // paged_weigh_kernel turns them into probabilities once the denominators are known.
 #include <algorithm>
+#include <cstring>
 
 #include "mma.cuh"
 #include "paged.cuh"
+#include "tc.cuh"
+#include "tensor_map.h"
 
 namespace cera {
 
+__device__ unsigned int g_paged_decode_status = 0;
+
+static const bool g_paged_decode_registered = register_kernel_status([] {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_paged_decode_status, sizeof(v));
+    return (uint32_t)v << 24;
+});
+
 namespace {
 
-constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_ROWS = 8;
+constexpr int PD_CTAS = 512;  // at most
+constexpr int PD_WARPS = 4, PD_MATH = 32 * PD_WARPS, PD_THREADS = PD_MATH + 64, PD_ROWS = 8;  // a warp for the keys and one for the values
 constexpr float PD_FLOOR = -3.0e38f;    // below every score that is a number
 constexpr float PD_LIFT = 7.0f;         // weights are 2^7 at the maximum's score, 2^15 at most
 constexpr float PD_RAISE = 8.0f;
+constexpr uint32_t PD_BEGIN = 2;
 
 struct PdParams {
     PagedView kv;
@@ -41,29 +56,42 @@ struct PdParams {
     float2 *ml;     // [2 G][8]: maximum, sum; then, with weights, [units][8]
     float *scores;  // [seqs][heads][capacity] or null
     float2 *ml_unit;
-    size_t cap;
+    size_t cap;                     // of scores, a multiple of 64
     float scale;
     uint32_t heads, group, chunks;  // chunks of eight heads in a group
-    bool same;                      // keys and values are laid out alike
+    uint32_t box;                   // slots a TMA copy brings
 };
 
-// The tiles of the call in one line; sums live in shared memory.
-struct PdLine {
-    const uint32_t *sums;  // visible tiles ahead of sequence s, of one unit each; sums[n] is all
-    uint32_t n, per_seq;   // units of a sequence
-};
+// The tiles that a query in the last of len slots sees: those that hold the first `sink` slots, then from the one with the window's first slot on.
+struct PdSpan {
+    uint32_t len, first, sinks, sink_tiles, skip, tiles;
 
-template <int KG>
-struct PdCursor {
-    uint32_t s, unit, tile, tiles, first, sinks, seen;
-
-    __device__ __forceinline__ void sequence(const PdLine &line, const PagedView &kv, const PagedMask &mask) {
-        tiles = line.sums[s + 1] - line.sums[s];
-        const uint32_t len = paged_len(kv, s);
-        first = len ? paged_first(mask, len - 1) : 0;
+    __device__ __forceinline__ void set(const PagedMask &mask, uint32_t n, uint32_t tile) {
+        len = n;
+        first = n ? paged_first(mask, n - 1) : 0;
         sinks = min(mask.sink, first);
-        seen = len - first + sinks;
+        skip = first / tile;
+        sink_tiles = min((sinks + tile - 1) / tile, skip);
+        skip -= sink_tiles;
+        tiles = (n + tile - 1) / tile - skip;
     }
+    __device__ __forceinline__ uint32_t slot(uint32_t t, uint32_t tile) const { return (t < sink_tiles ? t : t + skip) * tile; }
+    __device__ __forceinline__ bool sees(uint32_t j) const { return j < len && (j >= first || j < sinks); }
+};
+
+// The tiles of the call in one line, each unit's behind a stretch of PD_BEGIN that stands for what a unit costs beside its tiles (its queries, and
+// the warps' meeting at its end): without it a CTA that got many short units took twice as long as the rest (24 sequences of 1 to 9000 slots
+// TIME_A us, with it TIME_B).  Where every tile has a CTA of its own there is none.  sums live in shared memory.
+struct PdLine {
+    const uint32_t *sums;        // the line ahead of sequence s, of one unit each; sums[n] is all
+    uint32_t n, per_seq, begin;  // units of a sequence; a unit's stretch
+    __device__ __forceinline__ uint32_t length(uint32_t tiles) const { return tiles ? tiles + begin : 0; }
+};
+
+template <int TILE>
+struct PdCursor : PdSpan {
+    uint32_t s, unit, tile;
+
     __device__ __forceinline__ void seek(const PdLine &line, const PagedView &kv, const PagedMask &mask, uint64_t x) {
         uint32_t lo = 0, hi = line.n;  // the last s with sums[s] per_seq <= x, which has tiles
         while (hi - lo > 1) {
@@ -72,11 +100,14 @@ struct PdCursor {
             else hi = mid;
         }
         s = lo;
-        sequence(line, kv, mask);
+        set(mask, paged_len(kv, s), TILE);
         const uint64_t r = x - (uint64_t)line.sums[s] * line.per_seq;
-        unit = tiles ? (uint32_t)(r / tiles) : 0;
-        tile = tiles ? (uint32_t)(r - (uint64_t)unit * tiles) : 0;
+        const uint32_t all = max(line.length(tiles), 1u);
+        unit = (uint32_t)(r / all);
+        const uint32_t in = (uint32_t)(r - (uint64_t)unit * all);
+        tile = in > line.begin ? in - line.begin : 0;
     }
+    __device__ __forceinline__ bool behind(const PdCursor &o) const { return s != o.s ? s < o.s : unit != o.unit ? unit < o.unit : tile < o.tile; }
     __device__ __forceinline__ void step(const PdLine &line, const PagedView &kv, const PagedMask &mask) {
         if (++tile < tiles) return;
         tile = 0;
@@ -84,18 +115,17 @@ struct PdCursor {
         unit = 0;
         do ++s;
         while (s + 1 < line.n && line.sums[s + 1] == line.sums[s]);
-        if (s < line.n) sequence(line, kv, mask);
+        if (s < line.n) set(mask, paged_len(kv, s), TILE);
     }
-    __device__ __forceinline__ uint32_t slot(uint32_t x) const { return x < sinks ? x : x - sinks + first; }
 };
 
-__device__ __forceinline__ void cp_async16_or_zero(void *dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tma::smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One box of a tensor map of four dimensions, asked for by the lane for which `me` is true.  x * element size is a multiple of 16 bytes.
+__device__ __forceinline__ void tensor_g2s_4d_if(void *dst, const void *map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t *bar, uint32_t me) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(tma::smem_u32(dst)),
+        "l"(map), "r"(tma::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(me)
+        : "memory");
 }
 __device__ __forceinline__ float pd_exp2(float x) {
     float y;
@@ -103,30 +133,48 @@ __device__ __forceinline__ float pd_exp2(float x) {
     return y;
 }
 
-// The tiles ahead of each sequence, by the whole CTA.
-template <int KG>
-__device__ __forceinline__ PdLine pd_line(const PagedView &kv, const PagedMask &mask, uint32_t per_seq, uint32_t *sums, uint32_t *warps) {
+// The line, by the whole CTA.
+template <int TILE>
+__device__ __forceinline__ PdLine pd_line(const PagedView &kv, const PagedMask &mask, uint32_t per_seq, uint32_t ctas, uint32_t *sums, uint2 *warps) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, per = (kv.n_seqs + PD_THREADS - 1) / PD_THREADS, s0 = min(tid * per, kv.n_seqs), s1 = min(s0 + per, kv.n_seqs);
-    uint32_t mine = 0;
+    uint32_t tiles = 0, live = 0;
     for (uint32_t s = s0; s < s1; ++s) {
-        const uint32_t len = paged_len(kv, s), first = len ? paged_first(mask, len - 1) : 0;
-        mine += (len - first + min(mask.sink, first) + PD_WARPS * KG - 1) / (PD_WARPS * KG);
-        sums[s + 1] = mine;
+        PdSpan span;
+        span.set(mask, paged_len(kv, s), TILE);
+        sums[s + 1] = span.tiles;
+        tiles += span.tiles;
+        live += span.tiles != 0;
     }
-    uint32_t x = mine;
+    uint32_t x = tiles, y = live;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= (uint32_t)o) x += a;
+        const uint32_t a = __shfl_up_sync(0xffffffffu, x, o), b = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= (uint32_t)o) {
+            x += a;
+            y += b;
+        }
     }
-    if (lane == 31) warps[tid >> 5] = x;
+    if (lane == 31) warps[tid >> 5] = make_uint2(x, y);
     if (tid == 0) sums[0] = 0;
     __syncthreads();
-    uint32_t before = x - mine;
-    for (uint32_t w = 0; w < tid >> 5; ++w) before += warps[w];
-    for (uint32_t s = s0; s < s1; ++s) sums[s + 1] += before;
+    uint32_t all = 0;
+    x -= tiles;
+    y -= live;
+    for (uint32_t w = 0; w < PD_THREADS / 32; ++w) {
+        all += warps[w].x;
+        if (w < tid >> 5) {
+            x += warps[w].x;
+            y += warps[w].y;
+        }
+    }
+    PdLine line{sums, kv.n_seqs, per_seq, (uint64_t)all * per_seq > ctas ? PD_BEGIN : 0};
+    x += y * line.begin;
+    for (uint32_t s = s0; s < s1; ++s) {
+        x += line.length(sums[s + 1]);
+        sums[s + 1] = x;
+    }
     __syncthreads();
-    return PdLine{sums, kv.n_seqs, per_seq};
+    return line;
 }
 
 // ---- what a warp does with its keys of a tile ------------------------------------------------------------------------------
@@ -134,9 +182,10 @@ __device__ __forceinline__ PdLine pd_line(const PagedView &kv, const PagedMask &
 // 16-bit cache.  Lane = (row lane / 4, columns 2 (lane % 4) + {0, 1}) of an mma tile; acc's second half is the lower parts'.
 template <typename T, typename TQ, int DP>
 struct PdMma {
-    static constexpr int KG = 16, ROWB = DP * 2 + 16, CPR = DP / 8, QREGS = 1;
+    static constexpr int KG = 16, TILE = PD_WARPS * KG, BLOCK = 64;  // BLOCK: numbers of a 128-byte row
     static constexpr bool SPLIT = sizeof(TQ) == 4, BF = sizeof(T) == 2 && !std::is_same<T, __half>::value, THIRD = SPLIT && BF;
     uint32_t qf[DP / 16][SPLIT ? 4 : 2], q3[THIRD ? DP / 16 : 1][2];
+    uint32_t wf[4], w3[4];
     float acc[DP / 8][4], m, l, factor;
 
     static __device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -208,25 +257,28 @@ struct PdMma {
         l = 0.0f;
     }
 
-    // ks, vs: 16 rows each; mask: which are seen; scores: the first of these keys' places for head 0 of the unit, or null
-    __device__ __forceinline__ void tile(const PdParams &p, const uint8_t *ks, const uint8_t *vs, uint32_t mask, uint32_t rows, float *scores, uint32_t count, float *, float *) {
+    // ks: the tile's keys; mask: which of the warp's are seen; scores: the first of these keys' places for head 0 of the unit, or null
+    __device__ __forceinline__ void weigh(const PdParams &p, const uint8_t *ks, uint32_t mask, uint32_t rows, float *scores, const float *, float *) {
         const uint32_t lane = threadIdx.x & 31, r = lane >> 2, c2 = 2 * (lane & 3);
-        float sc[2][4] = {};
-        const uint8_t *ka = ks + ((lane & 7) + (lane >> 4) * 8) * ROWB + (lane >> 3 & 1) * 16;
+        float sc[2][4] = {}, sd[2][4] = {};  // two sums each: a product waits for the one before the last
+        const uint8_t *ka = ks + ((threadIdx.x >> 5) * KG + (lane & 7) + (lane >> 4) * 8) * 128;
+        const uint32_t turn = ((lane & 7) ^ (lane >> 3 & 1)) * 16;  // 16-byte chunk c of row i lies at c ^ i % 8
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
             if (k * 16 >= p.kv.dim) break;
             uint32_t b[4];
-            ldsm4(b, ka + k * 32);
+            ldsm4(b, ka + (k >> 2) * TILE * 128 + (turn ^ (k & 3) * 32));
             const uint32_t a[4] = {qf[k][0], SPLIT ? qf[k][SPLIT ? 2 : 0] : 0u, qf[k][1], SPLIT ? qf[k][SPLIT ? 3 : 1] : 0u};
-            mma(sc[0], a, b[0], b[1]);
-            mma(sc[1], a, b[2], b[3]);
+            mma(k & 1 ? sd[0] : sc[0], a, b[0], b[1]);
+            mma(k & 1 ? sd[1] : sc[1], a, b[2], b[3]);
             if (THIRD) {
                 const uint32_t a3[4] = {q3[THIRD ? k : 0][0], 0u, q3[THIRD ? k : 0][1], 0u};
-                mma(sc[0], a3, b[0], b[1]);
-                mma(sc[1], a3, b[2], b[3]);
+                mma(k & 1 ? sd[0] : sc[0], a3, b[0], b[1]);
+                mma(k & 1 ? sd[1] : sc[1], a3, b[2], b[3]);
             }
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[i >> 2][i & 3] += sd[i >> 2][i & 3];
         float z[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -241,8 +293,7 @@ struct PdMma {
         if (scores && r < rows) {
             float *to = scores + (size_t)r * p.cap + c2;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c2 + (i & 1) + (i >> 1) * 8 < count) to[(i & 1) + (i >> 1) * 8] = z[i];
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<float2 *>(to + 8 * i) = make_float2(z[2 * i], z[2 * i + 1]);
         }
         float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
         if (__any_sync(0xffffffffu, mx > m + PD_RAISE)) {
@@ -263,24 +314,28 @@ struct PdMma {
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pd_exp2(z[i] + base);
         l += (w[0] + w[1]) + (w[2] + w[3]);
-        uint32_t a[4], a3[4] = {0, 0, 0, 0};
-        split(w[0], w[1], a[0], a[1]);
-        split(w[2], w[3], a[2], a[3]);
+        split(w[0], w[1], wf[0], wf[1]);
+        split(w[2], w[3], wf[2], wf[3]);
         if (THIRD) {
-            a3[0] = third(w[0], w[1], a[0], a[1]);
-            a3[2] = third(w[2], w[3], a[2], a[3]);
+            w3[0] = third(w[0], w[1], wf[0], wf[1]);
+            w3[2] = third(w[2], w[3], wf[2], wf[3]);
+            w3[1] = w3[3] = 0;
         }
-        const uint8_t *va = vs + (lane & 15) * ROWB + (lane >> 4) * 16;
+    }
+    __device__ __forceinline__ void add(const PdParams &p, const uint8_t *vs, const float *) {
+        const uint32_t lane = threadIdx.x & 31;
+        const uint8_t *va = vs + ((threadIdx.x >> 5) * KG + (lane & 15)) * 128;
+        const uint32_t turn = ((lane & 7) ^ (lane >> 4)) * 16;
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
             if (n * 16 >= p.kv.dim) break;
             uint32_t b[4];
-            ldsm4_trans(b, va + n * 32);
-            mma(acc[2 * n], a, b[0], b[1]);
-            mma(acc[2 * n + 1], a, b[2], b[3]);
+            ldsm4_trans(b, va + (n >> 2) * TILE * 128 + (turn ^ (n & 3) * 32));
+            mma(acc[2 * n], wf, b[0], b[1]);
+            mma(acc[2 * n + 1], wf, b[2], b[3]);
             if (THIRD) {
-                mma(acc[2 * n], a3, b[0], b[1]);
-                mma(acc[2 * n + 1], a3, b[2], b[3]);
+                mma(acc[2 * n], w3, b[0], b[1]);
+                mma(acc[2 * n + 1], w3, b[2], b[3]);
             }
         }
     }
@@ -293,7 +348,7 @@ struct PdMma {
         if ((lane & 3) == 0) ml[lane >> 2] = make_float2(m, l);
     }
     // the weighted values for the maxima `all` of each row, [8][dim]
-    __device__ __forceinline__ void values(const PdParams &p, const float *all, float *to) {
+    __device__ __forceinline__ void values(const PdParams &p, const float *all, float *to) const {
         const uint32_t lane = threadIdx.x & 31, r = lane >> 2;
         const float f = pd_exp2(m - all[r]);
 #pragma unroll
@@ -313,7 +368,7 @@ struct PdMma {
 // f32 cache.  Scores: lane = (key lane / 4, every fourth 16 bytes of the row), then two heads of that key.  Values: lane = 4 dimensions.
 template <int DP>
 struct PdFma {
-    static constexpr int KG = 8, ROWB = DP * 4 + 64, CPR = DP / 4, NV = (DP + 127) / 128;
+    static constexpr int KG = 8, TILE = PD_WARPS * KG, BLOCK = 32, NV = (DP + 127) / 128;
     float4 acc[PD_ROWS][NV];
     float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1}; l over this lane's keys
 
@@ -334,14 +389,16 @@ struct PdFma {
         l[0] = l[1] = 0.0f;
     }
 
-    __device__ __forceinline__ void tile(const PdParams &p, const uint8_t *ks, const uint8_t *vs, uint32_t mask, uint32_t rows, float *scores, uint32_t count, float *qs, float *ps) {
+    __device__ __forceinline__ void weigh(const PdParams &p, const uint8_t *ks, uint32_t mask, uint32_t rows, float *scores, const float *qs, float *ps) {
         const uint32_t lane = threadIdx.x & 31, key = lane >> 2, part = lane & 3;
+        const uint8_t *ka = ks + ((threadIdx.x >> 5) * KG + key) * 128;
         float2 d2[PD_ROWS];
 #pragma unroll
         for (int r = 0; r < PD_ROWS; ++r) d2[r] = make_float2(0.0f, 0.0f);
 #pragma unroll 4
-        for (uint32_t c = part; c < p.kv.dim / 4; c += 4) {
-            const float4 k = *reinterpret_cast<const float4 *>(ks + key * ROWB + c * 16);
+        for (uint32_t i = 0; i < p.kv.dim / 16; ++i) {
+            const uint32_t c = part + 4 * (i ^ (key & 1));  // chunk c lies at c ^ key % 8: odd keys go the other way round, so that two meet all banks
+            const float4 k = *reinterpret_cast<const float4 *>(ka + (c >> 3) * TILE * 128 + ((c & 7) ^ key) * 16);
 #pragma unroll
             for (int r = 0; r < PD_ROWS; ++r) {
                 const float4 q = *reinterpret_cast<const float4 *>(qs + r * DP + c * 4);
@@ -366,7 +423,7 @@ struct PdFma {
             z[i] = (keep + __shfl_xor_sync(0xffffffffu, give, 1)) * (p.scale * PAGED_LOG2E);
         }
         if (!(mask >> key & 1)) z[0] = z[1] = -INFINITY;
-        if (scores && key < count) {
+        if (scores) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (2 * part + i < rows) scores[(size_t)(2 * part + i) * p.cap + key] = z[i];
@@ -400,6 +457,10 @@ struct PdFma {
         l[1] += w.y;
         *reinterpret_cast<float2 *>(ps + key * PD_ROWS + 2 * part) = w;
         __syncwarp();
+    }
+    __device__ __forceinline__ void add(const PdParams &p, const uint8_t *vs, const float *ps) {
+        const uint32_t lane = threadIdx.x & 31;
+        const uint8_t *va = vs + (threadIdx.x >> 5) * KG * 128;
 #pragma unroll
         for (int k = 0; k < KG; ++k) {
             const float4 w0 = *reinterpret_cast<const float4 *>(ps + k * PD_ROWS), w1 = *reinterpret_cast<const float4 *>(ps + k * PD_ROWS + 4);
@@ -407,7 +468,8 @@ struct PdFma {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if ((lane + 32 * i) * 4 >= p.kv.dim) break;
-                const float4 v = *reinterpret_cast<const float4 *>(vs + k * ROWB + (lane + 32 * i) * 16);
+                const uint32_t c = lane + 32 * i;
+                const float4 v = *reinterpret_cast<const float4 *>(va + (c >> 3) * TILE * 128 + k * 128 + ((c & 7) ^ k) * 16);
 #pragma unroll
                 for (int r = 0; r < PD_ROWS; ++r) {
                     const float2 wr = make_float2(ww[r], ww[r]);
@@ -417,7 +479,6 @@ struct PdFma {
                 }
             }
         }
-        __syncwarp();  // the weights' place is written by the next tile
     }
 
     __device__ __forceinline__ void end(float2 *ml) {
@@ -452,81 +513,132 @@ struct PdOf<float, float, DP> {
     using W = PdFma<DP>;
 };
 
-// Shared memory: rings | values of the warps at a unit's end | queries and weights (f32) | the line's sums.
+// Shared memory: the ring | values of the warps at a unit's end | queries and weights (f32) | the line's sums.
 template <typename W, int DP, int ST, bool FMA>
 struct PdSmem {
-    static constexpr size_t STAGE = 2 * (size_t)W::KG * W::ROWB, RING = ST * STAGE, VALUES = (size_t)PD_WARPS * PD_ROWS * DP * 4,
-                            EXTRA = FMA ? PD_WARPS * (size_t)(PD_ROWS * DP + PD_ROWS * W::KG) * 4 : 0, FIXED = PD_WARPS * RING + VALUES + EXTRA;
+    static constexpr size_t HALF = (size_t)W::TILE * DP * (FMA ? 4 : 2), STAGE = 2 * HALF, VALUES = (size_t)PD_WARPS * PD_ROWS * DP * 4,
+                            EXTRA = FMA ? PD_WARPS * (size_t)(PD_ROWS * DP + PD_ROWS * W::KG) * 4 : 0, FIXED = 1024 + ST * STAGE + VALUES + EXTRA;
 };
 
-template <typename T, typename TQ, int DP, int ST>
-__global__ void __launch_bounds__(PD_THREADS) paged_decode_kernel(const PdParams p) {
+__device__ __forceinline__ void pd_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PD_MATH) : "memory"); }  // the warps that compute
+
+template <typename T, typename TQ, int DP, int ST, bool TMA>
+__global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PdParams p) {
     using W = typename PdOf<T, TQ, DP>::W;
-    constexpr bool FMA = sizeof(T) == 4;
-    using S = PdSmem<W, DP, ST, FMA>;
-    constexpr int KG = W::KG, CPR = W::CPR;
-    extern __shared__ __align__(128) uint8_t smem[];
+    using S = PdSmem<W, DP, ST, sizeof(T) == 4>;
+    constexpr int KG = W::KG, TILE = W::TILE;
+    extern __shared__ uint8_t raw[];
     __shared__ float2 ml_s[PD_WARPS][PD_ROWS];
     __shared__ float all_s[PD_ROWS], sum_s[PD_ROWS];
-    __shared__ uint32_t mask_s[PD_WARPS][ST], scan_s[PD_WARPS], any_s[PD_WARPS];
+    __shared__ uint2 scan_s[PD_THREADS / 32];
+    __shared__ uint32_t mask_s[ST][2], any_s[PD_WARPS], abort_s;
+    __shared__ uint64_t full_s[2][ST], empty_s[ST];
+    uint8_t *smem = raw + (1024 - (tma::smem_u32(raw) & 1023)) % 1024;
+    float *values = reinterpret_cast<float *>(smem + ST * S::STAGE);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+    unsigned int *status = &g_paged_decode_status;
     pdl_trigger();
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            tma::mbar_init(&full_s[0][i], TMA ? 1 : 33);
+            tma::mbar_init(&full_s[1][i], TMA ? 1 : 33);
+            tma::mbar_init(&empty_s[i], PD_WARPS);
+        }
+        abort_s = 0;
+        tma::mbar_init_fence();
+    }
     pdl_wait();
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = gridDim.x, b = blockIdx.x;
-    uint8_t *ring = smem + warp * S::RING;
-    float *values = reinterpret_cast<float *>(smem + PD_WARPS * S::RING);
-    float *qs = values + PD_WARPS * PD_ROWS * DP + warp * (PD_ROWS * DP + PD_ROWS * KG), *ps = qs + PD_ROWS * DP;
     const uint32_t per_seq = p.kv.hk * p.chunks;
-    const PdLine line = pd_line<KG>(p.kv, p.mask, per_seq, reinterpret_cast<uint32_t *>(smem + S::FIXED), scan_s);
-    const uint64_t total = (uint64_t)line.sums[line.n] * per_seq, x0 = b * total / G, x1 = (b + 1) * total / G;
-    if (x0 >= x1) return;
-    PdCursor<KG> at, ahead;
+    const PdLine line = pd_line<TILE>(p.kv, p.mask, per_seq, gridDim.x, reinterpret_cast<uint32_t *>(smem + S::FIXED - 1024), scan_s);
+    const uint64_t total = (uint64_t)line.sums[line.n] * per_seq, parts = min((uint64_t)gridDim.x, total);
+    if (b >= parts) return;
+    const uint64_t x0 = b * total / parts, x1 = (b + 1) * total / parts;
+    PdCursor<TILE> at, end;
     at.seek(line, p.kv, p.mask, x0);
-    ahead = at;
+    end.seek(line, p.kv, p.mask, x1);  // the place behind everything, for the last CTA
+    if (!at.behind(end)) return;
 
-    // the row that this lane looks up for the tile at the cursor
-    auto find = [&](const PdCursor<KG> &c, uint32_t &page, uint32_t &row) {
-        const uint32_t x = (c.tile * PD_WARPS + warp) * KG + lane;
-        page = NO_PAGE;
-        row = 0;
-        if (lane < KG && x < c.seen) page = paged_at(p.kv, c.s, c.slot(x), row);
-    };
-    uint32_t page, row;
-    find(ahead, page, row);
-    uint64_t next = x0;
-    auto load = [&]() {
-        if (next < x1) {
-            const uint32_t st = (uint32_t)(next - x0) % ST;
-            uint8_t *kd = ring + st * S::STAGE, *vd = kd + KG * W::ROWB;
-            const uint32_t h = ahead.unit / p.chunks;
-            const bool there = page != NO_PAGE;
-            const uint64_t ko = there ? page * (uint64_t)p.kv.k_page + row * (uint64_t)p.kv.k_slot + h * (uint64_t)p.kv.k_head : 0;
-            const uint64_t vo = there ? page * (uint64_t)p.kv.v_page + row * (uint64_t)p.kv.v_slot + h * (uint64_t)p.kv.v_head : 0;
-            const uint32_t mask = __ballot_sync(0xffffffffu, there);
-            if (lane == 0) mask_s[warp][st] = mask;
-            ++next;
-            ahead.step(line, p.kv, p.mask);
-            if (next < x1) find(ahead, page, row);  // its answer is not needed before the next call
+    if (warp >= PD_WARPS) {
+        const bool is_v = warp > PD_WARPS;
+        uint64_t *full = full_s[is_v];
+        uint8_t *half = smem + (is_v ? S::HALF : 0);
+        const uint32_t boxes = TILE / p.box, blocks = (p.kv.dim + W::BLOCK - 1) / W::BLOCK;
+        const size_t by_page = is_v ? p.kv.v_page : p.kv.k_page, by_slot = is_v ? p.kv.v_slot : p.kv.k_slot, by_head = is_v ? p.kv.v_head : p.kv.k_head;
+        const uint8_t *base = is_v ? p.kv.v : p.kv.k;
+        // the pages of the tile at the cursor: with TMA lane i looks up box i, otherwise a lane the slots lane and lane + 32 of the tile
+        uint32_t page[2], row[2];
+        auto find = [&]() {
+            const uint32_t slot0 = at.slot(at.tile, TILE);
 #pragma unroll
-            for (int i = 0; i < KG * CPR / 32; ++i) {
-                const uint32_t idx = i * 32 + lane, r = idx / CPR, c = idx % CPR;
-                const uint64_t k1 = __shfl_sync(0xffffffffu, ko, r), v1 = p.same ? k1 : __shfl_sync(0xffffffffu, vo, r);
-                if (c * 16 < p.kv.dim * sizeof(T)) {
-                    const bool seen = mask >> r & 1;
-                    cp_async16_or_zero(kd + r * W::ROWB + c * 16, p.kv.k + k1 + (seen ? c * 16 : 0), seen);
-                    cp_async16_or_zero(vd + r * W::ROWB + c * 16, p.kv.v + v1 + (seen ? c * 16 : 0), seen);
+            for (int i = 0; i < 2; ++i) {
+                page[i] = NO_PAGE;
+                row[i] = 0;
+                if (TMA) {
+                    const uint32_t j = slot0 + lane * p.box;
+                    const bool some = j < at.len && (j + p.box > at.first || j < at.sinks);
+                    if (i == 0 && lane < boxes && some) page[0] = paged_at(p.kv, at.s, j, row[0]);
+                } else if (32 * i < TILE) {
+                    const uint32_t j = slot0 + lane + 32 * i;
+                    if (at.sees(j)) page[i] = paged_at(p.kv, at.s, j, row[i]);
                 }
             }
-        }
-        cp_async_commit();
-    };
+        };
+        find();
+        const uint32_t me = elect_one();
+        for (uint32_t x = 0; at.behind(end); ++x) {
+            const uint32_t st = x % ST;
+            const uint32_t slot0 = at.slot(at.tile, TILE), h = at.unit / p.chunks;
+            uint32_t mask[2];
+            uint32_t pg[2] = {page[0], page[1]}, rw[2] = {row[0], row[1]};
+            const uint32_t live = __ballot_sync(0xffffffffu, pg[0] != NO_PAGE);  // TMA: boxes
 #pragma unroll
-    for (int i = 0; i < ST; ++i) load();
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t j = lane + 32 * i;
+                const bool there = TMA ? j < TILE && at.sees(slot0 + j) && (live >> j / p.box & 1) : pg[i] != NO_PAGE;
+                mask[i] = __ballot_sync(0xffffffffu, there);
+            }
+            at.step(line, p.kv, p.mask);
+            if (at.behind(end)) find();  // its answer is not needed before the next tile
+            if (!tma::mbar_wait_warp(&empty_s[st], (x / ST & 1) ^ 1, &abort_s, status, 1u)) {  // given up: shared memory must outlive the copies in flight
+                for (uint32_t y = x > ST ? x - ST : 0; y < x; ++y)
+                    for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % ST], y / ST & 1); ++i) __nanosleep(40);
+                return;
+            }
+            if (!is_v && lane < 2) mask_s[st][lane] = lane ? mask[1] : mask[0];
+            __syncwarp();
+            uint8_t *to = half + st * S::STAGE;
+            if (TMA) {
+                tma::mbar_expect_tx_if(&full[st], __popc(live) * blocks * p.box * 128, me);
+                for (uint32_t i = 0; i < boxes; ++i) {
+                    const uint32_t pi = __shfl_sync(0xffffffffu, pg[0], i), ri = __shfl_sync(0xffffffffu, rw[0], i);
+                    if (pi == NO_PAGE) continue;
+                    for (uint32_t k = 0; k < blocks; ++k)
+                        tensor_g2s_4d_if(to + k * TILE * 128 + i * p.box * 128, is_v ? &map_v : &map_k, k * W::BLOCK, h, ri, pi, &full[st], me);
+                }
+            } else {
+                const uint32_t per = blocks * 8, used = p.kv.dim * sizeof(T) / 16;
+                uint64_t off[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) off[i] = pg[i] != NO_PAGE ? pg[i] * (uint64_t)by_page + rw[i] * (uint64_t)by_slot + h * (uint64_t)by_head : 0;
+                for (uint32_t i = lane; i < TILE * per; i += 32) {  // TILE * per is a multiple of 32: the warp stays together
+                    const uint32_t r = i / per, c = i - r * per;
+                    const uint64_t lo = __shfl_sync(0xffffffffu, off[0], r & 31), hi = __shfl_sync(0xffffffffu, off[1], r & 31);
+                    if (c < used && (mask[r >> 5] >> (r & 31) & 1))
+                        tma::cp_async16(to + (c >> 3) * TILE * 128 + r * 128 + ((c & 7) ^ (r & 7)) * 16, base + (r < 32 ? lo : hi) + c * 16);
+                }
+                tma::cp_async_arrive(&full[st]);
+                if (lane == 0) tma::mbar_arrive(&full[st]);  // the mask's
+            }
+        }
+        return;
+    }
 
+    float *qs = values + PD_WARPS * PD_ROWS * DP + warp * (PD_ROWS * DP + PD_ROWS * KG), *ps = qs + PD_ROWS * DP;
     W w;
-    uint32_t any = 0, first_tile = at.tile;
-    uint32_t rows = 0, head0 = 0;
-    for (uint64_t x = x0; x < x1; ++x) {
-        if (x == x0 || at.tile == 0) {
+    uint32_t any = 0, first_tile = at.tile, rows = 0, head0 = 0;
+    bool more = true;
+    for (uint32_t x = 0; more; ++x) {
+        if (x == 0 || at.tile == 0) {
             const uint32_t h = at.unit / p.chunks, c = at.unit - h * p.chunks;
             head0 = h * p.group + c * PD_ROWS;
             rows = min(p.group - c * PD_ROWS, (uint32_t)PD_ROWS);
@@ -534,23 +646,38 @@ __global__ void __launch_bounds__(PD_THREADS) paged_decode_kernel(const PdParams
             any = 0;
             w.begin(p, at.s, head0, rows, qs);
         }
-        const uint32_t st = (uint32_t)(x - x0) % ST, g0 = (at.tile * PD_WARPS + warp) * KG;
-        cp_async_wait<ST - 1>();
-        __syncwarp();
-        const uint32_t mask = mask_s[warp][st];
-        const uint8_t *ks = ring + st * S::STAGE;
+        const uint32_t st = x % ST, slot0 = at.slot(at.tile, TILE) + warp * KG;
+        const uint8_t *ks = smem + st * S::STAGE;
+        // a warp that gave up goes on without waiting; what it forms is reported as undefined
+        tma::mbar_wait_warp(&full_s[0][st], x / ST & 1, &abort_s, status, 2u);
+        const uint32_t mask = mask_s[st][warp * KG / 32] >> warp * KG % 32 & ((1u << KG) - 1);
         any |= mask;
-        const uint32_t count = g0 < at.seen ? min(at.seen - g0, (uint32_t)KG) : 0;
-        if (mask || (p.scores && count))
-            w.tile(p, ks, ks + KG * W::ROWB, mask, rows, p.scores ? p.scores + ((size_t)at.s * p.heads + head0) * p.cap + g0 : nullptr, count, qs, ps);
+        const bool work = mask || (p.scores && slot0 < at.len);
+        if (work) w.weigh(p, ks, mask, rows, p.scores ? p.scores + ((size_t)at.s * p.heads + head0) * p.cap + slot0 : nullptr, qs, ps);
+        tma::mbar_wait_warp(&full_s[1][st], x / ST & 1, &abort_s, status, 2u);
+        if (mask) {
+            uint8_t *vs = smem + st * S::STAGE + S::HALF;
+            if (mask != (1u << KG) - 1) {  // a weight of zero times what lies there could be a NaN
+                const uint32_t r = lane % KG;
+                if (!(mask >> r & 1))
+                    for (uint32_t c = lane / KG; c < DP * sizeof(T) / 16; c += 32 / KG)
+                        *reinterpret_cast<uint4 *>(vs + (c >> 3) * TILE * 128 + (warp * KG + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_smem();
+                __syncwarp();
+            }
+            w.add(p, vs, ps);
+        }
         __syncwarp();
-        load();
+        if (lane == 0) tma::mbar_arrive(&empty_s[st]);
+        const PdCursor<TILE> done = at;
         const bool last = at.tile + 1 == at.tiles;
-        if (last || x + 1 == x1) {
+        at.step(line, p.kv, p.mask);
+        more = at.behind(end);
+        if (last || !more) {
             // the warps' shares of the unit
             w.end(ml_s[warp]);
             if (lane == 0) any_s[warp] = any;
-            __syncthreads();
+            pd_sync();
             if (tid < PD_ROWS) {
                 float m = ml_s[0][tid].x, l = 0.0f;
                 for (int i = 1; i < PD_WARPS; ++i) m = fmaxf(m, ml_s[i][tid].x);
@@ -559,13 +686,13 @@ __global__ void __launch_bounds__(PD_THREADS) paged_decode_kernel(const PdParams
                 sum_s[tid] = l;
             }
             const bool seen = any_s[0] | any_s[1] | any_s[2] | any_s[3];
-            __syncthreads();
+            pd_sync();
             w.values(p, all_s, values + warp * PD_ROWS * p.kv.dim);
-            __syncthreads();
+            pd_sync();
             const bool whole = last && first_tile == 0;
-            const uint32_t slot = 2 * b + (x + 1 == x1 && x0 + (at.tile - first_tile) != x);  // the first unit of this CTA, or another, which is its last
-            const uint32_t n = PD_ROWS * p.kv.dim, unit = at.s * per_seq + at.unit;
-            for (uint32_t i = tid * 4; i < n; i += PD_THREADS * 4) {
+            const uint32_t slot = 2 * b + (done.tile - first_tile != x);  // the first unit of this CTA, or another, which is its last
+            const uint32_t n = PD_ROWS * p.kv.dim, unit = done.s * per_seq + done.unit;
+            for (uint32_t i = tid * 4; i < n; i += PD_MATH * 4) {
                 float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int k = 0; k < PD_WARPS; ++k) {
@@ -575,7 +702,7 @@ __global__ void __launch_bounds__(PD_THREADS) paged_decode_kernel(const PdParams
                 const uint32_t r = i / p.kv.dim;
                 if (whole) {
                     if (r < rows) {
-                        TQ *to = reinterpret_cast<TQ *>(p.out) + ((size_t)at.s * p.heads + head0) * p.kv.dim + i;
+                        TQ *to = reinterpret_cast<TQ *>(p.out) + ((size_t)done.s * p.heads + head0) * p.kv.dim + i;
                         const float f = sum_s[r];
                         to[0] = from_f32<TQ>(seen ? o.x / f : 0.0f);
                         to[1] = from_f32<TQ>(seen ? o.y / f : 0.0f);
@@ -591,72 +718,99 @@ __global__ void __launch_bounds__(PD_THREADS) paged_decode_kernel(const PdParams
                 if (!whole) p.ml[(size_t)slot * PD_ROWS + tid] = v;
                 else if (p.scores) p.ml_unit[(size_t)unit * PD_ROWS + tid] = v;
             }
-            __syncthreads();
+            pd_sync();
         }
-        at.step(line, p.kv, p.mask);
     }
-    cp_async_wait<0>();
 }
 
 // A CTA per (unit, row): units without tiles are zeros, whole ones are done, the others' parts are added up.
-template <typename TQ, int KG>
-__global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const PdParams p, uint32_t G) {
-    __shared__ uint32_t before_s[PD_WARPS], all_s[PD_WARPS], first_s;
+template <typename TQ, int TILE>
+__global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, uint32_t G) {
+    __shared__ uint4 sums_s[PD_WARPS];
+    __shared__ uint32_t first_s;
+    __shared__ float2 share_s[PD_CTAS];
+    __shared__ float max_s[PD_WARPS], sum_s[PD_WARPS];
+    __shared__ __align__(16) float value_s[PD_WARPS][256];
     pdl_trigger();
     pdl_wait();
     const uint32_t per_seq = p.kv.hk * p.chunks, unit = blockIdx.x, s = unit / per_seq, u = unit - s * per_seq, r = blockIdx.y, tid = threadIdx.x;
     const uint32_t h = u / p.chunks, c = u - h * p.chunks, rows = min(p.group - c * PD_ROWS, (uint32_t)PD_ROWS);
     if (r >= rows) return;
-    uint32_t before = 0, all = 0;
-    for (uint32_t i = tid; i < p.kv.n_seqs; i += PD_THREADS) {
-        const uint32_t len = paged_len(p.kv, i), first = len ? paged_first(p.mask, len - 1) : 0;
-        const uint32_t n = (len - first + min(p.mask.sink, first) + PD_WARPS * KG - 1) / (PD_WARPS * KG);
+    uint32_t before = 0, all = 0, live_before = 0, live = 0;  // sequences that have tiles count their stretch
+    for (uint32_t i = tid; i < p.kv.n_seqs; i += PD_MATH) {
+        PdSpan span;
+        span.set(p.mask, paged_len(p.kv, i), TILE);
+        const uint32_t n = span.tiles;
         all += n;
-        if (i < s) before += n;
+        live += n != 0;
+        if (i < s) {
+            before += n;
+            live_before += n != 0;
+        }
         if (i == s) first_s = n;
     }
     before = __reduce_add_sync(0xffffffffu, before);
     all = __reduce_add_sync(0xffffffffu, all);
-    if ((tid & 31) == 0) {
-        before_s[tid >> 5] = before;
-        all_s[tid >> 5] = all;
-    }
+    live_before = __reduce_add_sync(0xffffffffu, live_before);
+    live = __reduce_add_sync(0xffffffffu, live);
+    if ((tid & 31) == 0) sums_s[tid >> 5] = make_uint4(before, all, live_before, live);
     __syncthreads();
-    before = all = 0;
+    before = all = live_before = live = 0;
     for (int i = 0; i < PD_WARPS; ++i) {
-        before += before_s[i];
-        all += all_s[i];
+        before += sums_s[i].x;
+        all += sums_s[i].y;
+        live_before += sums_s[i].z;
+        live += sums_s[i].w;
     }
+    const uint32_t begin = (uint64_t)all * per_seq > G ? PD_BEGIN : 0;
+    all += live * begin;
+    before += live_before * begin;
     const uint32_t tiles = first_s;
     TQ *out = reinterpret_cast<TQ *>(p.out) + ((size_t)s * p.heads + h * p.group + c * PD_ROWS + r) * p.kv.dim;
     if (tiles == 0) {
-        for (uint32_t d = tid; d < p.kv.dim; d += PD_THREADS) out[d] = from_f32<TQ>(0.0f);
+        for (uint32_t d = tid; d < p.kv.dim; d += PD_MATH) out[d] = from_f32<TQ>(0.0f);
         return;
     }
-    const uint64_t total = (uint64_t)all * per_seq, u0 = (uint64_t)before * per_seq + (uint64_t)u * tiles, u1 = u0 + tiles;
-    const uint32_t b0 = (uint32_t)(((u0 + 1) * G - 1) / total), b1 = (uint32_t)((u1 * G - 1) / total);  // the CTAs of its first and last tile
+    const uint64_t total = (uint64_t)all * per_seq, parts = min((uint64_t)G, total), u0 = (uint64_t)before * per_seq + (uint64_t)u * (tiles + begin);
+    // the CTAs of its first and last tile: the last one that begins at or ahead of it
+    const uint32_t b0 = (uint32_t)(((u0 + begin + 1) * parts - 1) / total), b1 = (uint32_t)(((u0 + begin + tiles) * parts - 1) / total);
     if (b0 == b1) return;
-    const uint32_t head = 2 * b0 + (b0 * total / G < u0);  // of the first CTA it may be the last unit
-    auto slot = [&](uint32_t b) { return b == b0 ? head : 2 * b; };
-    auto empty = [&](uint32_t b) { return b * total / G == (b + 1) * total / G; };
+    const uint32_t n = b1 - b0 + 1, lane = tid & 31, warp = tid >> 5;
+    const uint32_t head = 2 * b0 + (b0 * total / parts < u0);  // of the first CTA it may be the last unit
+    auto slot = [&](uint32_t i) { return i ? 2 * (b0 + i) : head; };
     float m = -INFINITY, l = 0.0f;
-    for (uint32_t b = b0; b <= b1; ++b)
-        if (!empty(b)) m = fmaxf(m, p.ml[(size_t)slot(b) * PD_ROWS + r].x);
-    float o[2] = {0.0f, 0.0f};
-    for (uint32_t b = b0; b <= b1; ++b) {
-        if (empty(b)) continue;
-        const float2 v = p.ml[(size_t)slot(b) * PD_ROWS + r];
-        if (v.x == -INFINITY) continue;
-        const float f = pd_exp2(v.x - m);
-        l += v.y * f;
-        const float *part = p.part + ((size_t)slot(b) * PD_ROWS + r) * p.kv.dim;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (tid + i * PD_THREADS < p.kv.dim) o[i] = fmaf(part[tid + i * PD_THREADS], f, o[i]);
+    for (uint32_t i = tid; i < n; i += PD_MATH) {
+        const float2 v = p.ml[(size_t)slot(i) * PD_ROWS + r];
+        share_s[i] = v;
+        m = fmaxf(m, v.x);
     }
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) max_s[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(max_s[0], max_s[1]), fmaxf(max_s[2], max_s[3]));
+    float4 o[2] = {};
+#pragma unroll 4
+    for (uint32_t i = warp; i < n; i += PD_WARPS) {  // a warp a part, the warps' sums in their order
+        const float2 v = share_s[i];
+        const float f = v.x == -INFINITY ? 0.0f : pd_exp2(v.x - m);
+        const float *part = p.part + ((size_t)slot(i) * PD_ROWS + r) * p.kv.dim;
+        if (f == 0.0f) continue;
+        l = fmaf(v.y, f, l);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (tid + i * PD_THREADS < p.kv.dim) out[tid + i * PD_THREADS] = from_f32<TQ>(m == -INFINITY ? 0.0f : o[i] / l);
+        for (int k = 0; k < 2; ++k)
+            if (lane * 4 + k * 128 < p.kv.dim) {
+                const float4 a = *reinterpret_cast<const float4 *>(part + lane * 4 + k * 128);
+                o[k] = make_float4(fmaf(a.x, f, o[k].x), fmaf(a.y, f, o[k].y), fmaf(a.z, f, o[k].z), fmaf(a.w, f, o[k].w));
+            }
+    }
+    if (lane == 0) sum_s[warp] = l;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (lane * 4 + k * 128 < p.kv.dim) *reinterpret_cast<float4 *>(&value_s[warp][lane * 4 + k * 128]) = o[k];
+    __syncthreads();
+    l = sum_s[0] + sum_s[1] + sum_s[2] + sum_s[3];
+    for (uint32_t d = tid; d < p.kv.dim; d += PD_MATH)
+        out[d] = from_f32<TQ>(m == -INFINITY ? 0.0f : (value_s[0][d] + value_s[1][d] + value_s[2][d] + value_s[3][d]) / l);
     if (p.scores && tid == 0) p.ml_unit[(size_t)unit * PD_ROWS + r] = make_float2(m, l);
 }
 
@@ -669,18 +823,20 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PdParams p, floa
     const uint32_t first = paged_first(p.mask, len - 1), sinks = min(p.mask.sink, first), seen = len - first + sinks;
     const float *scores = p.scores + ((size_t)s * p.heads + h * p.group) * p.cap;
     for (uint32_t x = blockIdx.x * 256 + threadIdx.x; x < seen; x += gridDim.x * 256) {
+        const uint32_t slot = x < sinks ? x : x - sinks + first;
         float sum = 0.0f;
         for (uint32_t g = 0; g < p.group; ++g) {
             const float2 ml = p.ml_unit[((size_t)(s * p.kv.hk + h) * p.chunks + g / PD_ROWS) * PD_ROWS + g % PD_ROWS];
-            const float z = scores[(size_t)g * p.cap + x];
+            const float z = scores[(size_t)g * p.cap + slot];
             if (z != -INFINITY) sum += pd_exp2(z - ml.x + PD_LIFT) / ml.y;
         }
-        const uint32_t slot = x < sinks ? x : x - sinks + first;
         weights[((size_t)s * p.kv.hk + h) * stride + slot] += sum;
     }
 }
 
-uint32_t pd_grid() { return 2 * (uint32_t)sm_count(); }
+uint32_t pd_grid() { return std::min<uint32_t>(2 * (uint32_t)sm_count(), PD_CTAS); }
+
+size_t pd_cap(const PagedView &kv) { return ((size_t)kv.max_pages * kv.page_size + 63) / 64 * 64; }
 
 struct PdLayout {
     size_t part, ml, unit, scores, bytes;
@@ -692,21 +848,47 @@ PdLayout pd_layout(const PagedView &kv, size_t n_heads, bool weights) {
     l.ml = l.part + 2 * G * PD_ROWS * kv.dim * 4;
     l.unit = l.ml + 2 * G * PD_ROWS * 8;
     l.scores = l.unit + (weights ? kv.n_seqs * kv.hk * chunks * PD_ROWS * 8 : 0);
-    l.bytes = l.scores + (weights ? kv.n_seqs * n_heads * kv.max_pages * kv.page_size * 4 : 0) + 16;
+    l.bytes = l.scores + (weights ? kv.n_seqs * n_heads * pd_cap(kv) * 4 : 0) + 16;
     return l;
 }
 
+// The pages of keys or values as a tensor map: [pages][slots][heads][numbers], boxes of `box` slots and 128 bytes of one head.
+int32_t pd_map(CUtensorMap *map, int type, const void *base, const PagedView &kv, size_t page, size_t slot, size_t head, uint32_t box) {
+    const uint32_t e = type == CERA_TYPE_F32 ? 4 : 2;
+    const uint64_t dims[4] = {kv.dim, kv.hk, kv.page_size, kv.n_pages};
+    uint64_t strides[3] = {head, slot, page};
+    for (int i = 0; i < 3; ++i)
+        if (dims[i + 1] == 1) strides[i] = 16;  // nothing is that far
+    const uint32_t boxes[4] = {128 / e, 1, box, 1};
+    const CUtensorMapDataType t = type == CERA_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == CERA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return tensor_map_4d(map, t, base, dims, strides, boxes);
+}
+
 template <typename T, typename TQ, int DP, int ST>
-int32_t pd_launch(const PdParams &p, float *weights, size_t weights_stride, cudaStream_t st) {
+int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, cudaStream_t st) {
     using W = typename PdOf<T, TQ, DP>::W;
     const size_t smem = PdSmem<W, DP, ST, sizeof(T) == 4>::FIXED + ((size_t)p.kv.n_seqs + 1) * 4;
-    const size_t tiles = (p.cap + PD_WARPS * W::KG - 1) / (PD_WARPS * W::KG) * p.kv.n_seqs * p.kv.hk * p.chunks;
-    const uint32_t G = (uint32_t)std::min<size_t>(pd_grid(), std::max<size_t>(tiles, 1));
-    auto kernel = paged_decode_kernel<T, TQ, DP, ST>;
+    const size_t tiles = ((size_t)p.kv.max_pages * p.kv.page_size + W::TILE - 1) / W::TILE * p.kv.n_seqs * p.kv.hk * p.chunks;
+    const uint32_t G = (uint32_t)std::min<size_t>(DP <= 128 ? pd_grid() : pd_grid() / 2, std::max<size_t>(tiles, 1));  // what fits the SMs at once
+    CUtensorMap mk, mv;
+    memset(&mk, 0, sizeof(mk));
+    mv = mk;
+    // by TMA: a page holds whole boxes of at least a warp's keys
+    p.box = W::TILE;
+    while (p.box >= W::KG && p.kv.page_size % p.box) p.box /= 2;
+    const size_t far = std::max({p.kv.k_page, p.kv.k_slot, p.kv.k_head, p.kv.v_page, p.kv.v_slot, p.kv.v_head});
+    const bool by_tma = p.box >= W::KG && p.kv.n_pages && far < (1ull << 40);
+    if (by_tma) {
+        CERA_TRY(pd_map(&mk, type, p.kv.k, p.kv, p.kv.k_page, p.kv.k_slot, p.kv.k_head, p.box));
+        CERA_TRY(pd_map(&mv, type, p.kv.v, p.kv, p.kv.v_page, p.kv.v_slot, p.kv.v_head, p.box));
+    } else {
+        p.box = W::TILE;
+    }
+    auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, true> : paged_decode_kernel<T, TQ, DP, ST, false>;
     CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     count_launch(weights ? 3 : 2);
-    CERA_CUDA_TRY(launch_k(kernel, dim3(G), dim3(PD_THREADS), smem, st, p));
-    CERA_CUDA_TRY(launch_k(paged_join_kernel<TQ, W::KG>, dim3(p.kv.n_seqs * p.kv.hk * p.chunks, std::min<uint32_t>(p.group, PD_ROWS)), dim3(PD_THREADS), 0, st, p, G));
+    CERA_CUDA_TRY(launch_k(kernel, dim3(G), dim3(PD_THREADS), smem, st, mk, mv, p));
+    CERA_CUDA_TRY(launch_k(paged_join_kernel<TQ, W::TILE>, dim3(p.kv.n_seqs * p.kv.hk * p.chunks, std::min<uint32_t>(p.group, PD_ROWS)), dim3(PD_MATH), 0, st, p, G));
     if (!weights) return CERA_CUDA_OK;
     const uint32_t wide = (uint32_t)std::min<size_t>((p.cap + 255) / 256, std::max<size_t>(1, 148 * 8 / std::max(1u, p.kv.n_seqs * p.kv.hk)));
     return check_cuda(launch_k(paged_weigh_kernel, dim3(std::max(1u, wide), p.kv.hk, p.kv.n_seqs), dim3(256), 0, st, p, weights, weights_stride), "paged decode weights launch");
@@ -729,18 +911,17 @@ int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_
     p.ml = (float2 *)(w + lay.ml);
     p.ml_unit = (float2 *)(w + lay.unit);
     p.scores = weights ? (float *)(w + lay.scores) : nullptr;
-    p.cap = (size_t)kv.max_pages * kv.page_size;
+    p.cap = pd_cap(kv);
     p.scale = scale;
     p.heads = (uint32_t)n_heads;
     p.group = p.heads / kv.hk;
     p.chunks = (p.group + PD_ROWS - 1) / PD_ROWS;
-    p.same = kv.k_page == kv.v_page && kv.k_slot == kv.v_slot && kv.k_head == kv.v_head;
     auto go = [&](auto cache, auto query) {
         using T = decltype(cache);
         using TQ = decltype(query);
-        if (kv.dim <= 64) return pd_launch<T, TQ, 64, 3>(p, weights, weights_stride, st);
-        if (kv.dim <= 128) return pd_launch<T, TQ, 128, 2>(p, weights, weights_stride, st);
-        return pd_launch<T, TQ, 256, 2>(p, weights, weights_stride, st);
+        if (kv.dim <= 64) return pd_launch<T, TQ, 64, 3>(p, type, weights, weights_stride, st);
+        if (kv.dim <= 128) return pd_launch<T, TQ, 128, 2>(p, type, weights, weights_stride, st);
+        return pd_launch<T, TQ, 256, 2>(p, type, weights, weights_stride, st);
     };
     if (type == CERA_TYPE_F32) return go(float(), float());
     if (type == CERA_TYPE_F16) return q_type == type ? go(__half(), __half()) : go(__half(), float());

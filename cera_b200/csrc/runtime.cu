@@ -120,8 +120,7 @@ void scratch_trim() {
     cudaGetLastError();
 }
 
-int32_t tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t elem_bytes, const void *base, uint64_t rows, uint64_t ld, uint32_t box_cols,
-                      uint32_t box_rows, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -129,12 +128,31 @@ int32_t tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t elem_
             p = nullptr;
         return (PFN_cuTensorMapEncodeTiled_v12000)p;
     }();
+    return encode;
+}
+
+int32_t tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t elem_bytes, const void *base, uint64_t rows, uint64_t ld, uint32_t box_cols,
+                      uint32_t box_rows, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+    const auto encode = map_encoder();
     if (!encode) return fail(CERA_CUDA_ERR_CUDA, "the driver offers no cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {ld, rows}, strides[1] = {ld * elem_bytes};
     const cuuint32_t box[2] = {box_cols, box_rows}, es[2] = {1, 1};
     const CUresult r = encode(map, type, 2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(CERA_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled: error %d for [%llu x %llu]", (int)r, (unsigned long long)rows, (unsigned long long)ld);
+    return CERA_CUDA_OK;
+}
+
+int32_t tensor_map_4d(CUtensorMap *map, CUtensorMapDataType type, const void *base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                      const uint32_t (&box)[4]) {
+    const auto encode = map_encoder();
+    if (!encode) return fail(CERA_CUDA_ERR_CUDA, "the driver offers no cuTensorMapEncodeTiled");
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, s[3] = {strides[0], strides[1], strides[2]};
+    const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]}, es[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, type, 4, const_cast<void *>(base), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(CERA_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled: error %d for [%llu x %llu x %llu x %llu]", (int)r, (unsigned long long)dims[3],
+                                       (unsigned long long)dims[2], (unsigned long long)dims[1], (unsigned long long)dims[0]);
     return CERA_CUDA_OK;
 }
 
