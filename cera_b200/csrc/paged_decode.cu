@@ -79,6 +79,15 @@ struct PdSpan {
     __device__ __forceinline__ bool sees(uint32_t j) const { return j < len && (j >= first || j < sinks); }
 };
 
+// a / b; of numbers that fit 32 bits a short division, and they nearly always do.
+__device__ __forceinline__ uint32_t pd_div(uint64_t a, uint64_t b) { return (a | b) >> 32 ? (uint32_t)(a / b) : (uint32_t)a / (uint32_t)b; }
+
+// Where CTA b of `parts` begins on a line of `total`.
+__device__ __forceinline__ uint64_t pd_start(uint32_t b, uint64_t total, uint64_t parts) {
+    const uint64_t a = b * total;
+    return (a | parts) >> 32 ? a / parts : (uint32_t)a / (uint32_t)parts;
+}
+
 // The tiles of the call in one line, each unit's behind a stretch of PD_BEGIN that stands for what a unit costs beside its tiles (its queries, and
 // the warps' meeting at its end): without it a CTA that got many short units took twice as long as the rest (24 sequences of 1 to 9000 slots
 // TIME_A us, with it TIME_B).  Where every tile has a CTA of its own there is none.  sums live in shared memory.
@@ -103,7 +112,7 @@ struct PdCursor : PdSpan {
         set(mask, paged_len(kv, s), TILE);
         const uint64_t r = x - (uint64_t)line.sums[s] * line.per_seq;
         const uint32_t all = max(line.length(tiles), 1u);
-        unit = (uint32_t)(r / all);
+        unit = pd_div(r, all);
         const uint32_t in = (uint32_t)(r - (uint64_t)unit * all);
         tile = in > line.begin ? in - line.begin : 0;
     }
@@ -182,7 +191,7 @@ __device__ __forceinline__ PdLine pd_line(const PagedView &kv, const PagedMask &
 // 16-bit cache.  Lane = (row lane / 4, columns 2 (lane % 4) + {0, 1}) of an mma tile; acc's second half is the lower parts'.
 template <typename T, typename TQ, int DP>
 struct PdMma {
-    static constexpr int KG = 16, TILE = PD_WARPS * KG, BLOCK = 64;  // BLOCK: numbers of a 128-byte row
+    static constexpr int KG = 16, ROWS = PD_ROWS, TILE = PD_WARPS * KG, BLOCK = 64;  // BLOCK: numbers of a 128-byte row
     static constexpr bool SPLIT = sizeof(TQ) == 4, BF = sizeof(T) == 2 && !std::is_same<T, __half>::value, THIRD = SPLIT && BF;
     uint32_t qf[DP / 16][SPLIT ? 4 : 2], q3[THIRD ? DP / 16 : 1][2];
     uint32_t wf[4], w3[4];
@@ -366,72 +375,77 @@ struct PdMma {
 };
 
 // f32 cache.  Scores: lane = (key lane / 4, every fourth 16 bytes of the row), then two heads of that key.  Values: lane = 4 dimensions.
-template <int DP>
+template <int DP, int R>
 struct PdFma {
-    static constexpr int KG = 8, TILE = PD_WARPS * KG, BLOCK = 32, NV = (DP + 127) / 128;
-    float4 acc[PD_ROWS][NV];
-    float m[2], l[2];  // of heads 2 (lane % 4) + {0, 1}; l over this lane's keys
+    static constexpr int KG = 8, ROWS = R, NZ = R / 4, TILE = PD_WARPS * KG, BLOCK = 32, NV = (DP + 127) / 128;
+    float4 acc[R][NV];
+    float m[NZ], l[NZ];  // of heads NZ (lane % 4) + [0, NZ); l over this lane's keys
 
     __device__ __forceinline__ void begin(const PdParams &p, uint32_t s, uint32_t head0, uint32_t rows, float *qs) {
         const uint32_t lane = threadIdx.x & 31;
         const float *q = reinterpret_cast<const float *>(p.q) + ((size_t)s * p.heads + head0) * p.kv.dim;
         __syncwarp();
-        for (uint32_t i = lane; i < PD_ROWS * DP; i += 32) {
+        for (uint32_t i = lane; i < R * DP; i += 32) {
             const uint32_t r = i / DP, d = i % DP;
             qs[i] = r < rows && d < p.kv.dim ? q[r * p.kv.dim + d] : 0.0f;
         }
         __syncwarp();
 #pragma unroll
-        for (int r = 0; r < PD_ROWS; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int i = 0; i < NV; ++i) acc[r][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        m[0] = m[1] = PD_FLOOR;
-        l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NZ; ++i) {
+            m[i] = PD_FLOOR;
+            l[i] = 0.0f;
+        }
     }
 
     __device__ __forceinline__ void weigh(const PdParams &p, const uint8_t *ks, uint32_t mask, uint32_t rows, float *scores, const float *qs, float *ps) {
         const uint32_t lane = threadIdx.x & 31, key = lane >> 2, part = lane & 3;
         const uint8_t *ka = ks + ((threadIdx.x >> 5) * KG + key) * 128;
-        float2 d2[PD_ROWS];
+        float2 d2[R];
 #pragma unroll
-        for (int r = 0; r < PD_ROWS; ++r) d2[r] = make_float2(0.0f, 0.0f);
+        for (int r = 0; r < R; ++r) d2[r] = make_float2(0.0f, 0.0f);
 #pragma unroll 4
         for (uint32_t i = 0; i < p.kv.dim / 16; ++i) {
             const uint32_t c = part + 4 * (i ^ (key & 1));  // chunk c lies at c ^ key % 8: odd keys go the other way round, so that two meet all banks
             const float4 k = *reinterpret_cast<const float4 *>(ka + (c >> 3) * TILE * 128 + ((c & 7) ^ key) * 16);
 #pragma unroll
-            for (int r = 0; r < PD_ROWS; ++r) {
+            for (int r = 0; r < R; ++r) {
                 const float4 q = *reinterpret_cast<const float4 *>(qs + r * DP + c * 4);
                 d2[r] = __ffma2_rn(make_float2(k.x, k.y), make_float2(q.x, q.y), d2[r]);
                 d2[r] = __ffma2_rn(make_float2(k.z, k.w), make_float2(q.z, q.w), d2[r]);
             }
         }
-        float d[PD_ROWS];
+        float d[R];
 #pragma unroll
-        for (int r = 0; r < PD_ROWS; ++r) d[r] = d2[r].x + d2[r].y;
-        // sums over the four lanes of a key; lane `part` keeps heads 2 part, 2 part + 1
+        for (int r = 0; r < R; ++r) d[r] = d2[r].x + d2[r].y;
+        // sums over the four lanes of a key; lane `part` keeps heads NZ part + [0, NZ)
         const bool up2 = part & 2, up1 = part & 1;
-        float h4[4], z[2];
+        float h2[R / 2], z[NZ];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float give = up2 ? d[i] : d[4 + i], keep = up2 ? d[4 + i] : d[i];
-            h4[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+        for (int i = 0; i < R / 2; ++i) {
+            const float give = up2 ? d[i] : d[R / 2 + i], keep = up2 ? d[R / 2 + i] : d[i];
+            h2[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
         }
+        bool raise = false;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float give = up1 ? h4[i] : h4[2 + i], keep = up1 ? h4[2 + i] : h4[i];
+        for (int i = 0; i < NZ; ++i) {
+            const float give = up1 ? h2[i] : h2[NZ + i], keep = up1 ? h2[NZ + i] : h2[i];
             z[i] = (keep + __shfl_xor_sync(0xffffffffu, give, 1)) * (p.scale * PAGED_LOG2E);
+            if (!(mask >> key & 1)) z[i] = -INFINITY;
+            raise |= z[i] > m[i] + PD_RAISE;
         }
-        if (!(mask >> key & 1)) z[0] = z[1] = -INFINITY;
         if (scores) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (2 * part + i < rows) scores[(size_t)(2 * part + i) * p.cap + key] = z[i];
+            for (int i = 0; i < NZ; ++i)
+                if (NZ * part + i < rows) scores[(size_t)(NZ * part + i) * p.cap + key] = z[i];
         }
-        if (__any_sync(0xffffffffu, z[0] > m[0] + PD_RAISE || z[1] > m[1] + PD_RAISE)) {
-            float f[2];
+        if (__any_sync(0xffffffffu, raise)) {
+            float f[NZ];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NZ; ++i) {
                 float mx = z[i];
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
@@ -444,18 +458,18 @@ struct PdFma {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < PD_ROWS; ++r) {
-                const float g = __shfl_sync(0xffffffffu, f[r & 1], r >> 1);
+            for (int r = 0; r < R; ++r) {
+                const float g = __shfl_sync(0xffffffffu, f[r % NZ], r / NZ);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) acc[r][i] = make_float4(acc[r][i].x * g, acc[r][i].y * g, acc[r][i].z * g, acc[r][i].w * g);
             }
         }
-        float2 w;
-        w.x = pd_exp2(z[0] + (PD_LIFT - m[0]));
-        w.y = pd_exp2(z[1] + (PD_LIFT - m[1]));
-        l[0] += w.x;
-        l[1] += w.y;
-        *reinterpret_cast<float2 *>(ps + key * PD_ROWS + 2 * part) = w;
+#pragma unroll
+        for (int i = 0; i < NZ; ++i) {
+            const float w = pd_exp2(z[i] + (PD_LIFT - m[i]));
+            l[i] += w;
+            ps[key * R + NZ * part + i] = w;
+        }
         __syncwarp();
     }
     __device__ __forceinline__ void add(const PdParams &p, const uint8_t *vs, const float *ps) {
@@ -463,15 +477,16 @@ struct PdFma {
         const uint8_t *va = vs + (threadIdx.x >> 5) * KG * 128;
 #pragma unroll
         for (int k = 0; k < KG; ++k) {
-            const float4 w0 = *reinterpret_cast<const float4 *>(ps + k * PD_ROWS), w1 = *reinterpret_cast<const float4 *>(ps + k * PD_ROWS + 4);
-            const float ww[PD_ROWS] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            float ww[R];
+#pragma unroll
+            for (int r = 0; r < R; r += 4) *reinterpret_cast<float4 *>(ww + r) = *reinterpret_cast<const float4 *>(ps + k * R + r);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if ((lane + 32 * i) * 4 >= p.kv.dim) break;
                 const uint32_t c = lane + 32 * i;
                 const float4 v = *reinterpret_cast<const float4 *>(va + (c >> 3) * TILE * 128 + k * 128 + ((c & 7) ^ k) * 16);
 #pragma unroll
-                for (int r = 0; r < PD_ROWS; ++r) {
+                for (int r = 0; r < R; ++r) {
                     const float2 wr = make_float2(ww[r], ww[r]);
                     const float2 lo = __ffma2_rn(wr, make_float2(v.x, v.y), make_float2(acc[r][i].x, acc[r][i].y));
                     const float2 hi = __ffma2_rn(wr, make_float2(v.z, v.w), make_float2(acc[r][i].z, acc[r][i].w));
@@ -484,18 +499,18 @@ struct PdFma {
     __device__ __forceinline__ void end(float2 *ml) {
         const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NZ; ++i) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-            if (lane < 4) ml[2 * lane + i] = make_float2(m[i], l[i]);
+            if (lane < 4) ml[NZ * lane + i] = make_float2(m[i], l[i]);
         }
     }
     __device__ __forceinline__ void values(const PdParams &p, const float *all, float *to) {
         const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-        for (int r = 0; r < PD_ROWS; ++r) {
-            const float f = pd_exp2(__shfl_sync(0xffffffffu, m[r & 1], r >> 1) - all[r]);
+        for (int r = 0; r < R; ++r) {
+            const float f = pd_exp2(__shfl_sync(0xffffffffu, m[r % NZ], r / NZ) - all[r]);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if ((lane + 32 * i) * 4 < p.kv.dim)
@@ -504,27 +519,27 @@ struct PdFma {
     }
 };
 
-template <typename T, typename TQ, int DP>
+template <typename T, typename TQ, int DP, int R>
 struct PdOf {
     using W = PdMma<T, TQ, DP>;
 };
-template <int DP>
-struct PdOf<float, float, DP> {
-    using W = PdFma<DP>;
+template <int DP, int R>
+struct PdOf<float, float, DP, R> {
+    using W = PdFma<DP, R>;
 };
 
 // Shared memory: the ring | values of the warps at a unit's end | queries and weights (f32) | the line's sums.
 template <typename W, int DP, int ST, bool FMA>
 struct PdSmem {
-    static constexpr size_t HALF = (size_t)W::TILE * DP * (FMA ? 4 : 2), STAGE = 2 * HALF, VALUES = (size_t)PD_WARPS * PD_ROWS * DP * 4,
-                            EXTRA = FMA ? PD_WARPS * (size_t)(PD_ROWS * DP + PD_ROWS * W::KG) * 4 : 0, FIXED = 1024 + ST * STAGE + VALUES + EXTRA;
+    static constexpr size_t HALF = (size_t)W::TILE * DP * (FMA ? 4 : 2), STAGE = 2 * HALF, VALUES = (size_t)PD_WARPS * W::ROWS * DP * 4,
+                            EXTRA = FMA ? PD_WARPS * (size_t)W::ROWS * (DP + W::KG) * 4 : 0, FIXED = 1024 + ST * STAGE + VALUES + EXTRA;
 };
 
 __device__ __forceinline__ void pd_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PD_MATH) : "memory"); }  // the warps that compute
 
-template <typename T, typename TQ, int DP, int ST, bool TMA>
+template <typename T, typename TQ, int DP, int ST, int R, bool TMA>
 __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PdParams p) {
-    using W = typename PdOf<T, TQ, DP>::W;
+    using W = typename PdOf<T, TQ, DP, R>::W;
     using S = PdSmem<W, DP, ST, sizeof(T) == 4>;
     constexpr int KG = W::KG, TILE = W::TILE;
     extern __shared__ uint8_t raw[];
@@ -552,7 +567,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
     const PdLine line = pd_line<TILE>(p.kv, p.mask, per_seq, gridDim.x, reinterpret_cast<uint32_t *>(smem + S::FIXED - 1024), scan_s);
     const uint64_t total = (uint64_t)line.sums[line.n] * per_seq, parts = min((uint64_t)gridDim.x, total);
     if (b >= parts) return;
-    const uint64_t x0 = b * total / parts, x1 = (b + 1) * total / parts;
+    const uint64_t x0 = pd_start(b, total, parts), x1 = pd_start(b + 1, total, parts);
     PdCursor<TILE> at, end;
     at.seek(line, p.kv, p.mask, x0);
     end.seek(line, p.kv, p.mask, x1);  // the place behind everything, for the last CTA
@@ -633,7 +648,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
         return;
     }
 
-    float *qs = values + PD_WARPS * PD_ROWS * DP + warp * (PD_ROWS * DP + PD_ROWS * KG), *ps = qs + PD_ROWS * DP;
+    float *qs = values + PD_WARPS * R * DP + warp * R * (DP + KG), *ps = qs + R * DP;
     W w;
     uint32_t any = 0, first_tile = at.tile, rows = 0, head0 = 0;
     bool more = true;
@@ -678,7 +693,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
             w.end(ml_s[warp]);
             if (lane == 0) any_s[warp] = any;
             pd_sync();
-            if (tid < PD_ROWS) {
+            if (tid < R) {
                 float m = ml_s[0][tid].x, l = 0.0f;
                 for (int i = 1; i < PD_WARPS; ++i) m = fmaxf(m, ml_s[i][tid].x);
                 for (int i = 0; i < PD_WARPS; ++i) l += ml_s[i][tid].y * pd_exp2(ml_s[i][tid].x - m);
@@ -687,11 +702,11 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
             }
             const bool seen = any_s[0] | any_s[1] | any_s[2] | any_s[3];
             pd_sync();
-            w.values(p, all_s, values + warp * PD_ROWS * p.kv.dim);
+            w.values(p, all_s, values + warp * R * p.kv.dim);
             pd_sync();
             const bool whole = last && first_tile == 0;
             const uint32_t slot = 2 * b + (done.tile - first_tile != x);  // the first unit of this CTA, or another, which is its last
-            const uint32_t n = PD_ROWS * p.kv.dim, unit = done.s * per_seq + done.unit;
+            const uint32_t n = R * p.kv.dim, unit = done.s * per_seq + done.unit;
             for (uint32_t i = tid * 4; i < n; i += PD_MATH * 4) {
                 float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -710,10 +725,10 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
                         to[3] = from_f32<TQ>(seen ? o.w / f : 0.0f);
                     }
                 } else {
-                    *reinterpret_cast<float4 *>(p.part + (size_t)slot * n + i) = o;
+                    *reinterpret_cast<float4 *>(p.part + (size_t)slot * PD_ROWS * p.kv.dim + i) = o;
                 }
             }
-            if (tid < PD_ROWS) {
+            if (tid < R) {
                 const float2 v = make_float2(seen ? all_s[tid] : -INFINITY, sum_s[tid]);
                 if (!whole) p.ml[(size_t)slot * PD_ROWS + tid] = v;
                 else if (p.scores) p.ml_unit[(size_t)unit * PD_ROWS + tid] = v;
@@ -773,10 +788,10 @@ __global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, u
     }
     const uint64_t total = (uint64_t)all * per_seq, parts = min((uint64_t)G, total), u0 = (uint64_t)before * per_seq + (uint64_t)u * (tiles + begin);
     // the CTAs of its first and last tile: the last one that begins at or ahead of it
-    const uint32_t b0 = (uint32_t)(((u0 + begin + 1) * parts - 1) / total), b1 = (uint32_t)(((u0 + begin + tiles) * parts - 1) / total);
+    const uint32_t b0 = pd_div((u0 + begin + 1) * parts - 1, total), b1 = pd_div((u0 + begin + tiles) * parts - 1, total);
     if (b0 == b1) return;
     const uint32_t n = b1 - b0 + 1, lane = tid & 31, warp = tid >> 5;
-    const uint32_t head = 2 * b0 + (b0 * total / parts < u0);  // of the first CTA it may be the last unit
+    const uint32_t head = 2 * b0 + (pd_start(b0, total, parts) < u0);  // of the first CTA it may be the last unit
     auto slot = [&](uint32_t i) { return i ? 2 * (b0 + i) : head; };
     float m = -INFINITY, l = 0.0f;
     for (uint32_t i = tid; i < n; i += PD_MATH) {
@@ -864,9 +879,9 @@ int32_t pd_map(CUtensorMap *map, int type, const void *base, const PagedView &kv
     return tensor_map_4d(map, t, base, dims, strides, boxes);
 }
 
-template <typename T, typename TQ, int DP, int ST>
+template <typename T, typename TQ, int DP, int ST, int R>
 int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, cudaStream_t st) {
-    using W = typename PdOf<T, TQ, DP>::W;
+    using W = typename PdOf<T, TQ, DP, R>::W;
     const size_t smem = PdSmem<W, DP, ST, sizeof(T) == 4>::FIXED + ((size_t)p.kv.n_seqs + 1) * 4;
     const size_t tiles = ((size_t)p.kv.max_pages * p.kv.page_size + W::TILE - 1) / W::TILE * p.kv.n_seqs * p.kv.hk * p.chunks;
     const uint32_t G = (uint32_t)std::min<size_t>(DP <= 128 ? pd_grid() : pd_grid() / 2, std::max<size_t>(tiles, 1));  // what fits the SMs at once
@@ -884,7 +899,7 @@ int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, 
     } else {
         p.box = W::TILE;
     }
-    auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, true> : paged_decode_kernel<T, TQ, DP, ST, false>;
+    auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, R, true> : paged_decode_kernel<T, TQ, DP, ST, R, false>;
     CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     count_launch(weights ? 3 : 2);
     CERA_CUDA_TRY(launch_k(kernel, dim3(G), dim3(PD_THREADS), smem, st, mk, mv, p));
@@ -919,9 +934,17 @@ int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_
     auto go = [&](auto cache, auto query) {
         using T = decltype(cache);
         using TQ = decltype(query);
-        if (kv.dim <= 64) return pd_launch<T, TQ, 64, 3>(p, type, weights, weights_stride, st);
-        if (kv.dim <= 128) return pd_launch<T, TQ, 128, 2>(p, type, weights, weights_stride, st);
-        return pd_launch<T, TQ, 256, 2>(p, type, weights, weights_stride, st);
+        auto rows = [&](auto r) {
+            constexpr int R = decltype(r)::value;
+            if (kv.dim <= 64) return pd_launch<T, TQ, 64, 3, R>(p, type, weights, weights_stride, st);
+            if (kv.dim <= 128) return pd_launch<T, TQ, 128, 2, R>(p, type, weights, weights_stride, st);
+            return pd_launch<T, TQ, 256, 2, R>(p, type, weights, weights_stride, st);
+        };
+        // FMAs go by rows: half of eight where the group has no more
+        if constexpr (sizeof(T) == 4) {
+            if (p.group <= 4) return rows(std::integral_constant<int, 4>());
+        }
+        return rows(std::integral_constant<int, PD_ROWS>());
     };
     if (type == CERA_TYPE_F32) return go(float(), float());
     if (type == CERA_TYPE_F16) return q_type == type ? go(__half(), __half()) : go(__half(), float());
