@@ -1,4 +1,7 @@
 // C entries of the paged cache: what they refuse, and storing new rows.
+#include <algorithm>
+#include <cstring>
+
 #include "paged.cuh"
 
 namespace cera {
@@ -101,6 +104,25 @@ int32_t check_workspace(const char *what, const void *ws, size_t have, size_t ne
 
 }  // namespace
 
+int32_t paged_maps(const PagedView &kv, int type, uint32_t least, uint32_t *box, CUtensorMap *k, CUtensorMap *v) {
+    memset(k, 0, sizeof(*k));
+    memset(v, 0, sizeof(*v));
+    while (*box >= least && kv.page_size % *box) *box /= 2;
+    const size_t far = std::max({kv.k_page, kv.k_slot, kv.k_head, kv.v_page, kv.v_slot, kv.v_head});
+    if (*box < least || !kv.n_pages || far >= 1ull << 40) {
+        *box = 0;
+        return CERA_CUDA_OK;
+    }
+    const uint32_t e = type == CERA_TYPE_F32 ? 4 : 2, boxes[4] = {128 / e, 1, *box, 1};
+    const uint64_t dims[4] = {kv.dim, kv.hk, kv.page_size, kv.n_pages};
+    const CUtensorMapDataType t = type == CERA_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == CERA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    uint64_t ks[3] = {kv.k_head, kv.k_slot, kv.k_page}, vs[3] = {kv.v_head, kv.v_slot, kv.v_page};
+    for (int i = 0; i < 3; ++i)
+        if (dims[i + 1] == 1) ks[i] = vs[i] = 16;  // nothing is that far
+    CERA_TRY(tensor_map_4d(k, t, kv.k, dims, ks, boxes));
+    return tensor_map_4d(v, t, kv.v, dims, vs, boxes);
+}
+
 int32_t launch_paged_append(const PagedView &kv, int type, const void *k, const void *v, int src_type, const int32_t *starts, size_t n, float *weights,
                             int32_t *positions, size_t track_stride, const int32_t *token_pos, cudaStream_t st) {
     auto go = [&](auto cache, auto source) {
@@ -162,7 +184,7 @@ int32_t cera_cuda_paged_decode_attention(const cera_cuda_paged_kv *kv, const voi
 size_t cera_cuda_paged_prefill_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads, size_t n_tokens) {
     PagedView v;
     if (view("paged_prefill_attention", kv, &v) != CERA_CUDA_OK || check_heads("paged_prefill_attention", v, kv->type, kv->type, n_heads) != CERA_CUDA_OK) return 0;
-    return paged_prefill_workspace(v, n_heads, n_tokens);
+    return paged_prefill_workspace(v, kv->type, n_heads, n_tokens);
 }
 
 int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const void *q_dev, int32_t q_type, size_t n_heads, const int32_t *starts_dev,
@@ -176,7 +198,7 @@ int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const vo
     if (!starts_dev) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: no starts", what);
     if (n_tokens * (n_heads / v.hk) > 0x7fffffffu) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: %zu tokens", what, n_tokens);
     if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: queries or result null or off a 16-byte boundary", what);
-    CERA_TRY(check_workspace(what, workspace_dev, workspace_bytes, paged_prefill_workspace(v, n_heads, n_tokens)));
+    CERA_TRY(check_workspace(what, workspace_dev, workspace_bytes, paged_prefill_workspace(v, kv->type, n_heads, n_tokens)));
     return launch_paged_prefill(v, kv->type, q_dev, q_type, n_heads, starts_dev, n_tokens, scale, PagedMask{window, n_sink}, out_dev, workspace_dev,
                                 (cudaStream_t)stream);
 }

@@ -53,11 +53,28 @@ __device__ __forceinline__ uint32_t paged_seq_of(const int32_t *starts, uint32_t
 // First slot of the window of a query in slot p; slots [sinks, first) are not seen, where sinks = min(sink, first).
 __device__ __forceinline__ uint32_t paged_first(const PagedMask &m, uint32_t p) { return m.window && p + 1 > m.window ? p + 1 - m.window : 0; }
 
+// The tiles that queries in slots [p, n) see: those that hold the first `sink` slots, then from the one with the first slot of p's window on.
+struct PagedSpan {
+    uint32_t len, first, sinks, sink_tiles, skip, tiles;
+
+    __device__ __forceinline__ void set(const PagedMask &mask, uint32_t p, uint32_t n, uint32_t tile) {
+        len = n;
+        first = n ? paged_first(mask, p) : 0;
+        sinks = min(mask.sink, first);
+        skip = first / tile;
+        sink_tiles = min((sinks + tile - 1) / tile, skip);
+        skip -= sink_tiles;
+        tiles = (n + tile - 1) / tile - skip;
+    }
+    __device__ __forceinline__ void newest(const PagedMask &mask, uint32_t n, uint32_t tile) { set(mask, n ? n - 1 : 0, n, tile); }
+    __device__ __forceinline__ uint32_t slot(uint32_t t, uint32_t tile) const { return (t < sink_tiles ? t : t + skip) * tile; }
+    __device__ __forceinline__ bool sees(uint32_t j) const { return j < len && (j >= first || j < sinks); }
+};
+
 // Softmax(scale q K^T) V of one query head by one warp, in f32 and one pass over the slots that it sees, no other is read.  q and out: dim
-// numbers.  lse (optional): the logarithm to base 2 of the softmax's denominator, in units of the scaled scores.
+// numbers.
 template <typename T, typename TQ>
-__device__ __forceinline__ void paged_attend_row(const PagedView &kv, const PagedMask &mask, uint32_t s, uint32_t kvh, uint32_t p, const TQ *q, float scale, TQ *out,
-                                 float *lse) {
+__device__ __forceinline__ void paged_attend_row(const PagedView &kv, const PagedMask &mask, uint32_t s, uint32_t kvh, uint32_t p, const TQ *q, float scale, TQ *out) {
     const uint32_t lane = threadIdx.x & 31;
     float qv[8], acc[8];
 #pragma unroll
@@ -91,7 +108,6 @@ __device__ __forceinline__ void paged_attend_row(const PagedView &kv, const Page
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (32 * i < kv.dim) out[lane + 32 * i] = from_f32<TQ>(any ? acc[i] / l : 0.0f);
-    if (lse && lane == 0) *lse = any ? m + log2f(l) : INFINITY;
 }
 
 }  // namespace cera

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "tensor_map.h"
 
 namespace cera {
 
@@ -18,12 +19,19 @@ struct PagedMask {
     uint32_t window, sink;
 };
 
+// Tensor maps of the pages of keys and values, boxes of *box slots and 128 bytes of one head laid down with the 128-byte swizzle: *box, a power of two, is halved
+// until a page holds whole boxes.  0 where that would take it below `least`, or the pages are none or too far apart: no maps, rows are copied one by one.
+int32_t paged_maps(const PagedView &kv, int type, uint32_t least, uint32_t *box, CUtensorMap *k, CUtensorMap *v);
+
 int32_t launch_paged_append(const PagedView &kv, int type, const void *k, const void *v, int src_type, const int32_t *starts, size_t n, float *weights,
                             int32_t *positions, size_t track_stride, const int32_t *token_pos, cudaStream_t st);
 size_t paged_decode_workspace(const PagedView &kv, size_t n_heads, bool weights);
 int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, float scale, PagedMask mask, float *weights,
                             size_t weights_stride, void *out, void *ws, cudaStream_t st);
-size_t paged_prefill_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);
+size_t paged_prefill_workspace(const PagedView &kv, int type, size_t n_heads, size_t n_tokens);
+size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);  // 16-bit caches
+int32_t launch_paged_prefill_tc(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
+                                PagedMask mask, void *out, void *ws, cudaStream_t st);
 int32_t launch_paged_prefill(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
                              PagedMask mask, void *out, void *ws, cudaStream_t st);
 int32_t launch_paged_evict(const PagedView &kv, int type, const float *weights, const int32_t *positions, size_t track_stride, size_t budget, uint32_t n_sink,

@@ -21,12 +21,10 @@
 // With weights wanted the scaled scores are stored on the way (4 bytes a head and slot, beside the 2 dim that are read for it), and
 // paged_weigh_kernel turns them into probabilities once the denominators are known.
 #include <algorithm>
-#include <cstring>
 
 #include "mma.cuh"
 #include "paged.cuh"
 #include "tc.cuh"
-#include "tensor_map.h"
 
 namespace cera {
 
@@ -62,23 +60,6 @@ struct PdParams {
     uint32_t box;                   // slots a TMA copy brings
 };
 
-// The tiles that a query in the last of len slots sees: those that hold the first `sink` slots, then from the one with the window's first slot on.
-struct PdSpan {
-    uint32_t len, first, sinks, sink_tiles, skip, tiles;
-
-    __device__ __forceinline__ void set(const PagedMask &mask, uint32_t n, uint32_t tile) {
-        len = n;
-        first = n ? paged_first(mask, n - 1) : 0;
-        sinks = min(mask.sink, first);
-        skip = first / tile;
-        sink_tiles = min((sinks + tile - 1) / tile, skip);
-        skip -= sink_tiles;
-        tiles = (n + tile - 1) / tile - skip;
-    }
-    __device__ __forceinline__ uint32_t slot(uint32_t t, uint32_t tile) const { return (t < sink_tiles ? t : t + skip) * tile; }
-    __device__ __forceinline__ bool sees(uint32_t j) const { return j < len && (j >= first || j < sinks); }
-};
-
 // a / b; of numbers that fit 32 bits a short division, and they nearly always do.
 __device__ __forceinline__ uint32_t pd_div(uint64_t a, uint64_t b) { return (a | b) >> 32 ? (uint32_t)(a / b) : (uint32_t)a / (uint32_t)b; }
 
@@ -98,7 +79,7 @@ struct PdLine {
 };
 
 template <int TILE>
-struct PdCursor : PdSpan {
+struct PdCursor : PagedSpan {
     uint32_t s, unit, tile;
 
     __device__ __forceinline__ void seek(const PdLine &line, const PagedView &kv, const PagedMask &mask, uint64_t x) {
@@ -109,7 +90,7 @@ struct PdCursor : PdSpan {
             else hi = mid;
         }
         s = lo;
-        set(mask, paged_len(kv, s), TILE);
+        newest(mask, paged_len(kv, s), TILE);
         const uint64_t r = x - (uint64_t)line.sums[s] * line.per_seq;
         const uint32_t all = max(line.length(tiles), 1u);
         unit = pd_div(r, all);
@@ -124,18 +105,10 @@ struct PdCursor : PdSpan {
         unit = 0;
         do ++s;
         while (s + 1 < line.n && line.sums[s + 1] == line.sums[s]);
-        if (s < line.n) set(mask, paged_len(kv, s), TILE);
+        if (s < line.n) newest(mask, paged_len(kv, s), TILE);
     }
 };
 
-// One box of a tensor map of four dimensions, asked for by the lane for which `me` is true.  x * element size is a multiple of 16 bytes.
-__device__ __forceinline__ void tensor_g2s_4d_if(void *dst, const void *map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t *bar, uint32_t me) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
-        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(tma::smem_u32(dst)),
-        "l"(map), "r"(tma::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(me)
-        : "memory");
-}
 __device__ __forceinline__ float pd_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -148,8 +121,8 @@ __device__ __forceinline__ PdLine pd_line(const PagedView &kv, const PagedMask &
     const uint32_t tid = threadIdx.x, lane = tid & 31, per = (kv.n_seqs + PD_THREADS - 1) / PD_THREADS, s0 = min(tid * per, kv.n_seqs), s1 = min(s0 + per, kv.n_seqs);
     uint32_t tiles = 0, live = 0;
     for (uint32_t s = s0; s < s1; ++s) {
-        PdSpan span;
-        span.set(mask, paged_len(kv, s), TILE);
+        PagedSpan span;
+        span.newest(mask, paged_len(kv, s), TILE);
         sums[s + 1] = span.tiles;
         tiles += span.tiles;
         live += span.tiles != 0;
@@ -628,7 +601,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
                     const uint32_t pi = __shfl_sync(0xffffffffu, pg[0], i), ri = __shfl_sync(0xffffffffu, rw[0], i);
                     if (pi == NO_PAGE) continue;
                     for (uint32_t k = 0; k < blocks; ++k)
-                        tensor_g2s_4d_if(to + k * TILE * 128 + i * p.box * 128, is_v ? &map_v : &map_k, k * W::BLOCK, h, ri, pi, &full[st], me);
+                        tma::tensor_g2s_4d_if(to + k * TILE * 128 + i * p.box * 128, is_v ? &map_v : &map_k, k * W::BLOCK, h, ri, pi, &full[st], me);
                 }
             } else {
                 const uint32_t per = blocks * 8, used = p.kv.dim * sizeof(T) / 16;
@@ -753,8 +726,8 @@ __global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, u
     if (r >= rows) return;
     uint32_t before = 0, all = 0, live_before = 0, live = 0;  // sequences that have tiles count their stretch
     for (uint32_t i = tid; i < p.kv.n_seqs; i += PD_MATH) {
-        PdSpan span;
-        span.set(p.mask, paged_len(p.kv, i), TILE);
+        PagedSpan span;
+        span.newest(p.mask, paged_len(p.kv, i), TILE);
         const uint32_t n = span.tiles;
         all += n;
         live += n != 0;
@@ -867,18 +840,6 @@ PdLayout pd_layout(const PagedView &kv, size_t n_heads, bool weights) {
     return l;
 }
 
-// The pages of keys or values as a tensor map: [pages][slots][heads][numbers], boxes of `box` slots and 128 bytes of one head.
-int32_t pd_map(CUtensorMap *map, int type, const void *base, const PagedView &kv, size_t page, size_t slot, size_t head, uint32_t box) {
-    const uint32_t e = type == CERA_TYPE_F32 ? 4 : 2;
-    const uint64_t dims[4] = {kv.dim, kv.hk, kv.page_size, kv.n_pages};
-    uint64_t strides[3] = {head, slot, page};
-    for (int i = 0; i < 3; ++i)
-        if (dims[i + 1] == 1) strides[i] = 16;  // nothing is that far
-    const uint32_t boxes[4] = {128 / e, 1, box, 1};
-    const CUtensorMapDataType t = type == CERA_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == CERA_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return tensor_map_4d(map, t, base, dims, strides, boxes);
-}
-
 template <typename T, typename TQ, int DP, int ST, int R>
 int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, cudaStream_t st) {
     using W = typename PdOf<T, TQ, DP, R>::W;
@@ -886,19 +847,10 @@ int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, 
     const size_t tiles = ((size_t)p.kv.max_pages * p.kv.page_size + W::TILE - 1) / W::TILE * p.kv.n_seqs * p.kv.hk * p.chunks;
     const uint32_t G = (uint32_t)std::min<size_t>(DP <= 128 ? pd_grid() : pd_grid() / 2, std::max<size_t>(tiles, 1));  // what fits the SMs at once
     CUtensorMap mk, mv;
-    memset(&mk, 0, sizeof(mk));
-    mv = mk;
-    // by TMA: a page holds whole boxes of at least a warp's keys
     p.box = W::TILE;
-    while (p.box >= W::KG && p.kv.page_size % p.box) p.box /= 2;
-    const size_t far = std::max({p.kv.k_page, p.kv.k_slot, p.kv.k_head, p.kv.v_page, p.kv.v_slot, p.kv.v_head});
-    const bool by_tma = p.box >= W::KG && p.kv.n_pages && far < (1ull << 40);
-    if (by_tma) {
-        CERA_TRY(pd_map(&mk, type, p.kv.k, p.kv, p.kv.k_page, p.kv.k_slot, p.kv.k_head, p.box));
-        CERA_TRY(pd_map(&mv, type, p.kv.v, p.kv, p.kv.v_page, p.kv.v_slot, p.kv.v_head, p.box));
-    } else {
-        p.box = W::TILE;
-    }
+    CERA_TRY(paged_maps(p.kv, type, W::KG, &p.box, &mk, &mv));
+    const bool by_tma = p.box != 0;
+    if (!by_tma) p.box = W::TILE;
     auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, R, true> : paged_decode_kernel<T, TQ, DP, ST, R, false>;
     CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     count_launch(weights ? 3 : 2);

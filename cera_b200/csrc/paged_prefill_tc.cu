@@ -1,0 +1,735 @@
+// Causal attention of ragged prompt portions over a paged 16-bit cache on tcgen05, with a sliding window and first slots that stay visible.
+//
+// A row is (token, query head of a KV head), so a tile of 128 rows shares every staged key and value among the group's heads, whatever
+// their number.  A CTA owns up to two tiles of one (sequence, KV head) and walks tiles of KT keys: S = Q K^T into TMEM, softmax by a warpgroup a
+// tile (thread = row) in f32, P back into TMEM over S, O += P V with V as it lies in the cache (the product's transposed operand).  Two warps
+// load keys and values by TMA, a box of a page's slots an instruction (row by row where pages do not hold whole boxes), one warp
+// issues the products.  The tensor cores form one tile's products while the other tile's warpgroup is at its softmax.  The products of a tile
+// follow one another in the tensor pipe, so S of the next keys may go where P of these is still being read, and when S is complete O
+// is too: the warpgroup that finds a maximum raised by more than 2^8 rescales O on the spot.
+//
+// f32 queries over a 16-bit cache: the query and the weights enter as sums of NP parts of the cache's type (two f16, 22 bits; three
+// bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.
+//
+// Few rows over a long cache: the keys are split over gridDim.z CTAs and paged_prefill_join_kernel adds the parts up.
+//
+// A row that ends without finite values - a weight of zero times an infinite value of a key it does not see, an infinity cut into parts - or
+// that has met no weight is computed again by paged_attend_row, which reads nothing that the row does not see.  Every wait is bounded.
+#include <algorithm>
+
+#include "mma.cuh"
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace cera {
+
+__device__ unsigned int g_paged_prefill_status = 0;
+
+static const bool g_paged_prefill_registered = register_kernel_status([] {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_paged_prefill_status, sizeof(v));
+    return (uint32_t)v << 26;
+});
+
+namespace {
+
+constexpr uint32_t PP_ROWS = 128;
+constexpr float PP_FLOOR = -3.0e38f, PP_LIFT = 7.0f, PP_RAISE = 8.0f;
+constexpr uint32_t PP_MASKS = 4;  // tiles whose masks are kept: more than the keys' stages and one
+
+struct PpParams {
+    PagedView kv;
+    PagedMask mask;
+    const void *q;
+    const int32_t *starts;
+    void *out;
+    float *part;   // [splits][tokens][heads][dim], for splits > 1
+    float2 *ml;    // [splits][tokens][heads]
+    float scale;
+    uint32_t n, heads, group, box;
+};
+
+// Shapes by the padded head size and the number of parts.
+template <int DP, int NP>
+struct Pp {
+    static constexpr int MT = DP <= 128 ? 2 : 1;
+    static constexpr int KT = NP == 1 ? 128 : DP == 256 && NP == 3 ? 32 : 64;
+    static constexpr int BLOCKS = DP / 64;
+    static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
+    static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
+    static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((NP * P_COLS > KT ? NP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
+    static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 3);
+    static constexpr size_t SMEM = 1024 + (size_t)MT * NP * QPART + (size_t)ST * 2 * HALF;
+    static_assert(ST >= 1 && MT * T_COLS <= 512, "does not fit");
+};
+
+struct PpBars {
+    uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], o_full[2];
+};
+
+__device__ __forceinline__ float pp_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// D (+)= A[tmem] * B[smem], kind::f16.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t me) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(me)
+        : "memory");
+}
+// A tile of values as the product's second operand, rows of its k (keys) and numbers of its n contiguous: 8-row groups 1024 bytes apart, 64-number
+// blocks `block` bytes apart.
+__device__ __forceinline__ uint64_t pp_desc_v(uint32_t addr, uint32_t block) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint32_t pp_idesc(bool bf, uint32_t N, bool n_major) {
+    return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((n_major ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((PP_ROWS >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t pp_low(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pp_pack(float x, float y) {
+    if (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 pp_unpack(uint32_t w) {
+    if (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
+}
+// (x, y) as a sum of NP pairs of T.
+template <typename T, int NP>
+__device__ __forceinline__ void pp_parts(float x, float y, uint32_t (&w)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        w[i] = pp_pack<T>(x, y);
+        if (i + 1 < NP) {
+            const float2 f = pp_unpack<T>(w[i]);
+            x -= f.x;
+            y -= f.y;
+        }
+    }
+}
+
+// What a CTA works on: rows [row0, row0 + MT 128) of a (sequence, KV head), and of the key tiles that some of them sees [x0, x1).
+struct PpWork {
+    uint32_t s, row0, rows, t0, len;  // t0: the sequence's first token
+    int32_t p0;                       // the slot of its first token, negative if it has none
+    PagedSpan span;
+    uint32_t x0, x1;
+
+    __device__ __forceinline__ int32_t slot_of(uint32_t row, uint32_t group) const { return p0 + (int32_t)(row / group); }
+};
+
+// The unit-th run of MT tiles of all sequences, by a warp; false: there are not that many.
+template <int DP, int NP>
+__device__ __forceinline__ bool pp_find(const PpParams &p, PpWork &w, uint32_t unit) {
+    using C = Pp<DP, NP>;
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t ahead = 0;
+    for (uint32_t base = 0; base < p.kv.n_seqs; base += 32) {
+        const uint32_t s = base + lane;
+        uint32_t rows = 0;
+        if (s < p.kv.n_seqs) {
+            const int32_t a = min(max(p.starts[s], 0), (int32_t)p.n), b = min(max(p.starts[s + 1], a), (int32_t)p.n);
+            rows = (uint32_t)(b - a) * p.group;
+        }
+        const uint32_t units = (rows + C::MT * PP_ROWS - 1) / (C::MT * PP_ROWS);
+        uint32_t x = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, ahead + x > unit);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            w.s = base + src;
+            w.rows = __shfl_sync(0xffffffffu, rows, src);
+            const uint32_t first = ahead + __shfl_sync(0xffffffffu, x - units, src), n = __shfl_sync(0xffffffffu, units, src);
+            w.row0 = (n - 1 - (unit - first)) * C::MT * PP_ROWS;  // the last rows see the most: first
+            return true;
+        }
+        ahead += __shfl_sync(0xffffffffu, x, 31);
+    }
+    return false;
+}
+
+template <int DP, int NP>
+__device__ __forceinline__ void pp_set(const PpParams &p, PpWork &w) {
+    using C = Pp<DP, NP>;
+    w.t0 = (uint32_t)min(max(p.starts[w.s], 0), (int32_t)p.n);
+    w.len = paged_len(p.kv, w.s);
+    w.p0 = (int32_t)w.len - (int32_t)(w.rows / p.group);
+    const uint32_t last = min(w.row0 + C::MT * PP_ROWS, w.rows) - 1;
+    const int32_t lo = max(w.slot_of(w.row0, p.group), 0), hi = w.slot_of(last, p.group) + 1;
+    w.span.set(p.mask, (uint32_t)lo, (uint32_t)max(hi, 0), C::KT);
+    w.x0 = (uint32_t)((uint64_t)w.span.tiles * blockIdx.z / gridDim.z);
+    w.x1 = (uint32_t)((uint64_t)w.span.tiles * (blockIdx.z + 1) / gridDim.z);
+}
+
+// Whether tile t of the CTA's rows sees something of the key tile at slot0.
+template <int DP, int NP>
+__device__ __forceinline__ bool pp_sees(const PpParams &p, const PpWork &w, uint32_t t, uint32_t slot0) {
+    const uint32_t a = w.row0 + t * PP_ROWS;
+    if (a >= w.rows) return false;
+    const int32_t hi = w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group);
+    if (hi < (int32_t)slot0) return false;
+    const uint32_t first = paged_first(p.mask, (uint32_t)max(w.slot_of(a, p.group), 0));
+    return slot0 + Pp<DP, NP>::KT > first || slot0 < p.mask.sink;
+}
+
+// The keys' or the values' loader, a warp.
+template <typename T, int DP, int NP, bool TMA>
+__device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, const CUtensorMap *map, bool is_v, uint8_t *stages, uint64_t *full, uint64_t *empty,
+                                        uint32_t (*masks)[4], volatile uint32_t *abort_flag, unsigned int *status) {
+    using C = Pp<DP, NP>;
+    const uint32_t lane = threadIdx.x & 31, h = blockIdx.y, boxes = C::KT / p.box, blocks = (p.kv.dim + 63) / 64, me = elect_one();
+    const size_t by_page = is_v ? p.kv.v_page : p.kv.k_page, by_slot = is_v ? p.kv.v_slot : p.kv.k_slot, by_head = is_v ? p.kv.v_head : p.kv.k_head;
+    const uint8_t *base = is_v ? p.kv.v : p.kv.k;
+    constexpr int N = (C::KT + 31) / 32;
+    uint32_t page[N], row[N];
+    // with TMA lane i looks up box i, otherwise a lane the slots lane, lane + 32 ... of the tile
+    auto find = [&](uint32_t x) {
+        const uint32_t slot0 = w.span.slot(x, C::KT);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            page[i] = NO_PAGE;
+            row[i] = 0;
+            if (TMA) {
+                const uint32_t j = slot0 + lane * p.box;
+                if (i == 0 && lane < boxes && j < w.span.len && (j + p.box > w.span.first || j < w.span.sinks)) page[0] = paged_at(p.kv, w.s, j, row[0]);
+            } else {
+                const uint32_t j = slot0 + lane + 32 * i;
+                if (w.span.sees(j)) page[i] = paged_at(p.kv, w.s, j, row[i]);
+            }
+        }
+    };
+    if (w.x0 < w.x1) find(w.x0);
+    for (uint32_t x = w.x0; x < w.x1; ++x) {
+        const uint32_t i0 = x - w.x0, st = i0 % C::ST, slot0 = w.span.slot(x, C::KT);
+        uint32_t pg[N], rw[N], mask[N];
+        const uint32_t live = __ballot_sync(0xffffffffu, page[0] != NO_PAGE);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            pg[i] = page[i];
+            rw[i] = row[i];
+            const uint32_t j = lane + 32 * i;
+            mask[i] = __ballot_sync(0xffffffffu, TMA ? w.span.sees(slot0 + j) && (live >> j / p.box & 1) : pg[i] != NO_PAGE);
+        }
+        if (x + 1 < w.x1) find(x + 1);  // its answer is not needed before the next tile
+        if (!tma::mbar_wait_warp(&empty[st], (i0 / C::ST & 1) ^ 1, abort_flag, status, 1u)) {  // given up: shared memory must outlive the copies in flight
+            for (uint32_t y = i0 > C::ST ? i0 - C::ST : 0; y < i0; ++y)
+                for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % C::ST], y / C::ST & 1); ++i) __nanosleep(40);
+            return;
+        }
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (lane == (uint32_t)i) masks[i0 % PP_MASKS][i] = mask[i];
+        }
+        __syncwarp();
+        uint8_t *to = stages + st * C::HALF;
+        if (TMA) {
+            tma::mbar_expect_tx_if(&full[st], __popc(live) * blocks * p.box * 128, me);
+            for (uint32_t i = 0; i < boxes; ++i) {
+                const uint32_t pi = __shfl_sync(0xffffffffu, pg[0], i), ri = __shfl_sync(0xffffffffu, rw[0], i);
+                if (pi == NO_PAGE) continue;
+                for (uint32_t k = 0; k < blocks; ++k) tma::tensor_g2s_4d_if(to + k * C::KBLOCK + i * p.box * 128, map, k * 64, h, ri, pi, &full[st], me);
+            }
+        } else {
+            const uint32_t per = blocks * 8, used = p.kv.dim / 8;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint64_t off = pg[n] != NO_PAGE ? pg[n] * (uint64_t)by_page + rw[n] * (uint64_t)by_slot + h * (uint64_t)by_head : 0;
+                for (uint32_t i = lane; i < 32 * per; i += 32) {
+                    const uint32_t r = i / per, c = i - r * per;
+                    const uint64_t o = __shfl_sync(0xffffffffu, off, r);
+                    if (c < used && (mask[n] >> r & 1)) tma::cp_async16(to + (c >> 3) * C::KBLOCK + (32 * n + r) * 128 + ((c & 7) ^ (r & 7)) * 16, base + o + c * 16);
+                }
+            }
+            // what these copies write is read by the tensor cores: complete, fenced, then announced
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive(&full[st]);
+        }
+    }
+}
+
+// The products, a warp.
+template <typename T, int DP, int NP>
+__device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, uint8_t *qs, uint8_t *ks, uint8_t *vs, uint32_t tmem, PpBars *b, const uint32_t (*masks)[4],
+                                            volatile uint32_t *abort_flag, unsigned int *status) {
+    using C = Pp<DP, NP>;
+    constexpr bool BF = !std::is_same<T, __half>::value;
+    const uint32_t lane = threadIdx.x & 31, me = elect_one(), id_s = pp_idesc(BF, C::KT, false), id_o = pp_idesc(BF, p.kv.dim, true), n = w.x1 - w.x0;
+    auto arrived = [&](uint64_t *bar, uint32_t parity) { return tma::mbar_wait_warp(bar, parity, abort_flag, status, 2u); };
+    auto slot0 = [&](uint32_t i) { return w.span.slot(w.x0 + i, C::KT); };
+    uint32_t scored[2] = {0, 0}, added[2] = {0, 0};
+    auto score = [&](uint32_t t, uint32_t i) {
+        const uint32_t d = tmem + t * C::T_COLS;
+        const uint64_t kd = smem_desc_sw128(tma::smem_u32(ks + i % C::ST * C::HALF));
+        uint32_t acc = 0;
+        for (int part = 0; part < NP; ++part) {
+            const uint64_t qd = smem_desc_sw128(tma::smem_u32(qs + (t * NP + part) * C::QPART));
+            for (uint32_t k = 0; k < p.kv.dim / 16; ++k, acc = 1)
+                tc_mma_f16(d, qd + (k >> 2) * (C::QBLOCK / 16) + 2 * (k & 3), kd + (k >> 2) * (C::KBLOCK / 16) + 2 * (k & 3), id_s, acc, me);
+        }
+        tc_commit(&b->s_full[t], me);
+        ++scored[t];
+    };
+    if (n == 0 || !arrived(&b->q_full, 0) || !arrived(&b->k_full[0], 0)) return;
+    tc_fence_after();
+    for (uint32_t t = 0; t < C::MT; ++t)
+        if (pp_sees<DP, NP>(p, w, t, slot0(0))) score(t, 0);
+    tc_commit(&b->k_empty[0], me);
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint32_t st = i % C::ST, next = (i + 1) % C::ST;
+        bool there = false, ready = false;
+        uint8_t *vt = vs + st * C::HALF;
+        for (uint32_t t = 0; t < C::MT; ++t) {
+            if (pp_sees<DP, NP>(p, w, t, slot0(i))) {
+                if (!arrived(&b->p_full[t], added[t] & 1)) return;
+                if (!there) {
+                    if (!arrived(&b->v_full[st], i / C::ST & 1)) return;
+                    there = true;
+                    // rows that were not loaded: a weight of zero times what lies there could be a NaN
+                    bool fixed = false;
+#pragma unroll
+                    for (int m = 0; m < (C::KT + 31) / 32; ++m) {
+                        const uint32_t mask = masks[i % PP_MASKS][m];
+                        if (mask == 0xffffffffu) continue;
+                        fixed = true;
+                        for (uint32_t r = 0; r < 32; ++r)
+                            if (!(mask >> r & 1))
+                                for (uint32_t c = lane; c < DP / 8; c += 32) *reinterpret_cast<uint4 *>(vt + (c >> 3) * C::KBLOCK + (32 * m + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    if (fixed) {
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                const uint32_t o = tmem + t * C::T_COLS + C::S_COLS;
+                const uint64_t vd = pp_desc_v(tma::smem_u32(vt), C::KBLOCK);
+                for (int part = 0; part < NP; ++part)
+                    for (uint32_t k = 0; k < C::KT / 16; ++k)
+                        tc_mma_f16_ts(o, tmem + t * C::T_COLS + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
+                ++added[t];
+            }
+            if (i + 1 < n && pp_sees<DP, NP>(p, w, t, slot0(i + 1))) {
+                if (!ready) {
+                    if (!arrived(&b->k_full[next], (i + 1) / C::ST & 1)) return;
+                    tc_fence_after();
+                    ready = true;
+                }
+                score(t, i + 1);
+            }
+        }
+        // a stage that no tile of rows saw has to have arrived before it is filled again
+        if (!there && !arrived(&b->v_full[st], i / C::ST & 1)) return;
+        tc_commit(&b->v_empty[st], me);
+        if (i + 1 < n) {
+            if (!ready && !arrived(&b->k_full[next], (i + 1) / C::ST & 1)) return;
+            tc_commit(&b->k_empty[next], me);
+        }
+    }
+    for (uint32_t t = 0; t < C::MT; ++t) tc_commit(&b->o_full[t], me);
+}
+
+// A tile's queries into shared memory, a thread a row -> the factor of its scores, in units of ln 2.
+template <typename T, typename TQ, int DP, int NP>
+__device__ __forceinline__ float pp_queries(const PpParams &p, const PpWork &w, uint32_t row, uint8_t *to, uint32_t r) {
+    using C = Pp<DP, NP>;
+    const bool live = row < w.rows;
+    const TQ *q = reinterpret_cast<const TQ *>(p.q) + ((size_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group) * p.kv.dim;
+    float factor = fmaxf(fabsf(p.scale) * PAGED_LOG2E, 1.2e-38f);  // at a scale of zero all weights are alike, but for those of minus infinity
+    const bool turn = p.scale < 0.0f;
+    if (NP == 1) {
+        const uint32_t flip = turn ? 0x80008000u : 0;
+        for (uint32_t c = 0; c < p.kv.dim / 8; ++c) {
+            uint4 v = live ? reinterpret_cast<const uint4 *>(q)[c] : make_uint4(0, 0, 0, 0);
+            v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            *reinterpret_cast<uint4 *>(to + (c >> 3) * C::QBLOCK + r * 128 + ((c & 7) ^ (r & 7)) * 16) = v;
+        }
+        return factor;
+    }
+    float mul = turn ? -1.0f : 1.0f;
+    if (std::is_same<T, __half>::value) {
+        float most = 0.0f;
+        for (uint32_t c = 0; c < p.kv.dim / 4 && live; ++c) {
+            const float4 v = reinterpret_cast<const float4 *>(q)[c];
+            most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+        const int e = most > 0.0f && most <= 3.4e38f ? min(max((int)(__float_as_uint(most) >> 23 & 255) - 127, -120), 120) : 0;
+        mul *= __uint_as_float((uint32_t)(127 - e) << 23);
+        factor *= __uint_as_float((uint32_t)(127 + e) << 23);
+    }
+    for (uint32_t c = 0; c < p.kv.dim / 8; ++c) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 v = live ? reinterpret_cast<const float4 *>(q)[2 * c + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[4 * i] = v.x * mul;
+            x[4 * i + 1] = v.y * mul;
+            x[4 * i + 2] = v.z * mul;
+            x[4 * i + 3] = v.w * mul;
+        }
+        uint32_t u[4][NP];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pp_parts<T, NP>(x[2 * i], x[2 * i + 1], u[i]);
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+            *reinterpret_cast<uint4 *>(to + k * C::QPART + (c >> 3) * C::QBLOCK + r * 128 + ((c & 7) ^ (r & 7)) * 16) = make_uint4(u[0][k], u[1][k], u[2][k], u[3][k]);
+    }
+    return factor;
+}
+
+// Softmax and result of a tile of rows, a warpgroup.
+template <typename T, typename TQ, int DP, int NP>
+__device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, uint32_t t, uint8_t *qs, uint32_t tmem, PpBars *b, const uint32_t (*masks)[4],
+                                           volatile uint32_t *abort_flag, unsigned int *status) {
+    using C = Pp<DP, NP>;
+    constexpr int CH = NP == 1 ? 32 : C::KT;  // columns taken at a time: P goes over columns of S that have been read
+    const uint32_t lane = threadIdx.x & 31, quad = threadIdx.x >> 5 & 3, r = quad * 32 + lane, row = w.row0 + t * PP_ROWS + r;
+    const uint32_t ts = tmem + t * C::T_COLS + (quad * 32 << 16), to = ts + C::S_COLS;
+    const float c = pp_queries<T, TQ, DP, NP>(p, w, row, qs + t * NP * C::QPART, r);
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) tma::mbar_arrive(&b->q_full);
+
+    const uint32_t a = w.row0 + t * PP_ROWS, z = min(a + PP_ROWS, w.rows);
+    const bool live = row < w.rows;
+    const int32_t pos = live ? w.slot_of(row, p.group) : -1;
+    const int32_t p_lo = a < w.rows ? w.slot_of(a, p.group) : -1, p_hi = a < w.rows ? w.slot_of(z - 1, p.group) : -1;
+    const int32_t first = pos >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)pos) : 0, first_hi = p_hi >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)p_hi) : 0;
+    const int32_t sinks = (int32_t)min(p.mask.sink, (uint32_t)max(first, 0));
+    float m = PP_FLOOR, l = 0.0f;
+    uint32_t done = 0;
+    bool ok = true;
+    for (uint32_t i = 0; i < w.x1 - w.x0; ++i) {
+        const uint32_t slot0 = w.span.slot(w.x0 + i, C::KT);
+        if (!pp_sees<DP, NP>(p, w, t, slot0)) continue;
+        ok = tma::mbar_wait_warp(&b->s_full[t], done & 1, abort_flag, status, 4u);
+        if (!ok) break;
+        tc_fence_after();
+        // which of the tile's keys this row sees; nothing to look at where every row sees all
+        uint32_t see[(C::KT + 31) / 32];
+        bool all = (int32_t)(slot0 + C::KT) <= p_lo + 1 && ((int32_t)slot0 >= first_hi || slot0 + C::KT <= p.mask.sink);
+#pragma unroll
+        for (int k = 0; k < (C::KT + 31) / 32; ++k) {
+            see[k] = masks[i % PP_MASKS][k];
+            all = all && see[k] == 0xffffffffu;
+        }
+        if (!all) {
+#pragma unroll
+            for (int k = 0; k < (C::KT + 31) / 32; ++k) {
+                const int32_t at = (int32_t)slot0 + 32 * k;
+                see[k] &= pp_low(pos + 1 - at) & (~pp_low(first - at) | pp_low(sinks - at));
+            }
+        }
+        float mx = -INFINITY;
+        uint32_t v[CH / 32][32];
+#pragma unroll
+        for (int k = 0; k < C::KT / CH; ++k) {
+#pragma unroll
+            for (int j = 0; j < CH / 32; ++j) tmem_ld32(ts + k * CH + 32 * j, v[j]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < CH / 32; ++j) {
+                if (!all) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[j][e] = see[k * (CH / 32) + j] >> e & 1 ? v[j][e] : 0xff800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[j][e]));
+            }
+        }
+        mx *= c;
+        float f = 1.0f;
+        if (mx > m + PP_RAISE) {
+            f = pp_exp2(m - mx);
+            m = mx;
+            l *= f;
+        }
+        if (done && __any_sync(0xffffffffu, f != 1.0f)) {  // O is complete up to the tile before, and nothing adds to it
+            for (uint32_t d = 0; d < p.kv.dim; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + d, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(to + d, *reinterpret_cast<const uint32_t(*)[16]>(o));
+                tmem_st16(to + d + 16, *reinterpret_cast<const uint32_t(*)[16]>(o + 16));
+            }
+        }
+        const float base = PP_LIFT - m;
+#pragma unroll
+        for (int k = 0; k < C::KT / CH; ++k) {
+            if (C::KT > CH) {  // not in registers any more
+#pragma unroll
+                for (int j = 0; j < CH / 32; ++j) tmem_ld32(ts + k * CH + 32 * j, v[j]);
+                tmem_wait_ld();
+                if (!all) {
+#pragma unroll
+                    for (int j = 0; j < CH / 32; ++j)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[j][e] = see[k * (CH / 32) + j] >> e & 1 ? v[j][e] : 0xff800000u;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < CH / 32; ++j) {
+                uint32_t wd[NP][16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = pp_exp2(fmaf(__uint_as_float(v[j][2 * e]), c, base)), y = pp_exp2(fmaf(__uint_as_float(v[j][2 * e + 1]), c, base));
+                    l += x + y;
+                    uint32_t u[NP];
+                    pp_parts<T, NP>(x, y, u);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) wd[n][e] = u[n];
+                }
+#pragma unroll
+                for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + k * (CH / 2) + 16 * j, wd[n]);
+            }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tma::mbar_arrive(&b->p_full[t]);
+        ++done;
+    }
+    if (ok && done) ok = tma::mbar_wait_warp(&b->o_full[t], 0, abort_flag, status, 4u);
+    if (!ok) return;
+    tc_fence_after();
+    const size_t place = ((size_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group);
+    if (gridDim.z > 1) {
+        const size_t at = (size_t)blockIdx.z * p.n * p.heads + place;
+        if (live) p.ml[at] = make_float2(l > 0.0f || l != l || m != PP_FLOOR ? m : -INFINITY, l);
+        if (done)
+            for (uint32_t d = 0; d < p.kv.dim; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + d, o);
+                tmem_wait_ld();
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(p.part + at * p.kv.dim + d + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+        return;
+    }
+    TQ *out = reinterpret_cast<TQ *>(p.out) + place * p.kv.dim;
+    const float f = 1.0f / l;
+    float check = l > 0.0f ? 0.0f : NAN;
+    for (uint32_t d = 0; d < p.kv.dim; d += 32) {
+        uint32_t o[32];
+        if (done) {
+            tmem_ld32(to + d, o);
+            tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 16 / sizeof(TQ)) {
+            alignas(16) TQ y[16 / sizeof(TQ)];
+#pragma unroll
+            for (uint32_t k = 0; k < 16 / sizeof(TQ); ++k) {
+                const float x = done ? __uint_as_float(o[e + k]) * f : 0.0f;
+                check = fmaf(x, 0.0f, check);
+                y[k] = from_f32<TQ>(pos >= 0 ? x : 0.0f);
+            }
+            if (live) *reinterpret_cast<uint4 *>(out + d + e) = *reinterpret_cast<const uint4 *>(y);
+        }
+    }
+    uint32_t again = __ballot_sync(0xffffffffu, pos >= 0 && check != 0.0f);
+    for (; again; again &= again - 1) {
+        const uint32_t rr = a + quad * 32 + __ffs(again) - 1;
+        const size_t pl = ((size_t)(w.t0 + rr / p.group) * p.heads + blockIdx.y * p.group + rr % p.group) * p.kv.dim;
+        __syncwarp();
+        paged_attend_row<T, TQ>(p.kv, p.mask, w.s, blockIdx.y, (uint32_t)w.slot_of(rr, p.group), reinterpret_cast<const TQ *>(p.q) + pl, p.scale,
+                                reinterpret_cast<TQ *>(p.out) + pl);
+    }
+}
+
+template <typename T, typename TQ, int DP, int NP, bool TMA>
+__global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                                  const PpParams p) {
+    using C = Pp<DP, NP>;
+    extern __shared__ uint8_t raw[];
+    __shared__ PpBars bars;
+    __shared__ uint32_t masks[PP_MASKS][4], tmem_at, abort_s;
+    __shared__ PpWork work;
+    uint8_t *qs = raw + (1024 - (tma::smem_u32(raw) & 1023)) % 1024, *ks = qs + C::MT * NP * C::QPART, *vs = ks + C::ST * C::HALF;
+    const uint32_t warp = threadIdx.x >> 5;
+    pdl_trigger();
+    pdl_wait();
+    if (warp == 0) {
+        PpWork w;
+        const bool found = pp_find<DP, NP>(p, w, blockIdx.x);
+        if (found) pp_set<DP, NP>(p, w);
+        else w.rows = 0;
+        if (threadIdx.x == 0) {
+            work = w;
+            abort_s = 0;
+            tma::mbar_init(&bars.q_full, C::MATH);
+            for (int i = 0; i < 3; ++i) {
+                tma::mbar_init(&bars.k_full[i], 1);
+                tma::mbar_init(&bars.v_full[i], 1);
+                tma::mbar_init(&bars.k_empty[i], 1);
+                tma::mbar_init(&bars.v_empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                tma::mbar_init(&bars.s_full[i], 1);
+                tma::mbar_init(&bars.p_full[i], 4);
+                tma::mbar_init(&bars.o_full[i], 1);
+            }
+            tma::mbar_init_fence();
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    const PpWork w = work;
+    if (w.rows == 0) return;
+    if (warp == C::MATH) {
+        tmem_alloc(&tmem_at, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    unsigned int *status = &g_paged_prefill_status;
+    if (warp < C::MATH) {
+        pp_softmax<T, TQ, DP, NP>(p, w, warp / 4, qs, tmem, &bars, masks, &abort_s, status);
+    } else if (warp == C::MATH) {
+        pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, masks, &abort_s, status);
+    } else {
+        const bool is_v = warp == C::MATH + 2;
+        pp_load<T, DP, NP, TMA>(p, w, is_v ? &map_v : &map_k, is_v, is_v ? vs : ks, is_v ? bars.v_full : bars.k_full, is_v ? bars.v_empty : bars.k_empty, masks, &abort_s, status);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::MATH) tmem_dealloc(tmem, 512);
+}
+
+// A warp per row: the parts of its splits added up in their order.
+template <typename T, typename TQ>
+__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams p, uint32_t splits) {
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31;
+    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = (size_t)p.n * p.heads;
+    if (r >= all) return;
+    const uint32_t t = (uint32_t)(r / p.heads), h = (uint32_t)(r % p.heads), s = paged_seq_of(p.starts, p.kv.n_seqs, t);
+    if (s >= p.kv.n_seqs) return;
+    TQ *out = reinterpret_cast<TQ *>(p.out) + r * p.kv.dim;
+    const uint32_t len = paged_len(p.kv, s), behind = (uint32_t)p.starts[s + 1] - t;
+    if (behind > len) {
+        for (uint32_t d = lane; d < p.kv.dim; d += 32) out[d] = from_f32<TQ>(0.0f);
+        return;
+    }
+    float m = -INFINITY, l = 0.0f, o[8] = {};
+    for (uint32_t z = lane; z < splits; z += 32) m = fmaxf(m, p.ml[z * all + r].x);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+#pragma unroll 4
+    for (uint32_t z = 0; z < splits; ++z) {
+        const float2 v = p.ml[z * all + r];
+        if (v.x == -INFINITY) continue;
+        const float f = pp_exp2(v.x - m), *part = p.part + (z * all + r) * p.kv.dim;
+        l = fmaf(v.y, f, l);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (32 * i < p.kv.dim) o[i] = fmaf(part[lane + 32 * i], f, o[i]);
+    }
+    float check = l > 0.0f ? 0.0f : NAN;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (32 * i < p.kv.dim) {
+            check = fmaf(o[i] / l, 0.0f, check);
+            out[lane + 32 * i] = from_f32<TQ>(o[i] / l);
+        }
+    if (__any_sync(0xffffffffu, check != 0.0f))
+        paged_attend_row<T, TQ>(p.kv, p.mask, s, h / p.group, len - behind, reinterpret_cast<const TQ *>(p.q) + r * p.kv.dim, p.scale, out);
+}
+
+// CTAs along the rows (an upper bound: the portions' lengths are on the device) and the splits of the keys: as many as fill the SMs, of
+// four tiles of keys at least.
+struct PpGrid {
+    uint32_t units, splits;
+};
+PpGrid pp_grid(const PagedView &kv, size_t n_heads, size_t n) {
+    const size_t group = n_heads / kv.hk, rows = (kv.dim <= 128 ? 2 : 1) * PP_ROWS, units = std::min<size_t>(n * group / rows + std::min<size_t>(kv.n_seqs, n), n * group);
+    const size_t ctas = units * kv.hk, fit = (size_t)sm_count() / std::max<size_t>(ctas, 1), deep = (size_t)kv.max_pages * kv.page_size / 512;
+    return {(uint32_t)units, (uint32_t)std::max<size_t>(1, std::min(fit, deep))};
+}
+
+template <typename T, typename TQ, int DP>
+int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
+    constexpr int NP = sizeof(TQ) == 2 ? 1 : std::is_same<T, __half>::value ? 2 : 3;
+    using C = Pp<DP, NP>;
+    const PpGrid g = pp_grid(p.kv, p.heads, p.n);
+    CUtensorMap mk, mv;
+    p.box = C::KT;
+    CERA_TRY(paged_maps(p.kv, type, 8, &p.box, &mk, &mv));
+    const bool by_tma = p.box != 0;
+    if (!by_tma) p.box = C::KT;
+    auto kernel = by_tma ? paged_prefill_tc_kernel<T, TQ, DP, NP, true> : paged_prefill_tc_kernel<T, TQ, DP, NP, false>;
+    CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    count_launch(g.splits > 1 ? 2 : 1);
+    CERA_CUDA_TRY(launch_k(kernel, dim3(g.units, p.kv.hk, g.splits), dim3(C::THREADS), C::SMEM, st, mk, mv, p));
+    if (g.splits == 1) return CERA_CUDA_OK;
+    return check_cuda(launch_k(paged_prefill_join_kernel<T, TQ>, dim3((uint32_t)(((size_t)p.n * p.heads + 3) / 4)), dim3(128), 0, st, p, g.splits), "paged prefill join launch");
+}
+
+}  // namespace
+
+size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n) {
+    const PpGrid g = pp_grid(kv, n_heads, n);
+    return 16 + (g.splits > 1 ? g.splits * n * n_heads * ((size_t)kv.dim * 4 + 8) : 0);
+}
+
+int32_t launch_paged_prefill_tc(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
+                                PagedMask mask, void *out, void *ws, cudaStream_t st) {
+    PpParams p;
+    p.kv = kv;
+    p.mask = mask;
+    p.q = q;
+    p.starts = starts;
+    p.out = out;
+    p.scale = scale;
+    p.n = (uint32_t)n_tokens;
+    p.heads = (uint32_t)n_heads;
+    p.group = p.heads / kv.hk;
+    p.part = (float *)ws;
+    p.ml = (float2 *)((uint8_t *)ws + (size_t)pp_grid(kv, n_heads, n_tokens).splits * n_tokens * n_heads * kv.dim * 4);
+    auto go = [&](auto cache, auto query) {
+        using T = decltype(cache);
+        using TQ = decltype(query);
+        if (kv.dim <= 64) return pp_launch<T, TQ, 64>(p, type, st);
+        if (kv.dim <= 128) return pp_launch<T, TQ, 128>(p, type, st);
+        return pp_launch<T, TQ, 256>(p, type, st);
+    };
+    if (type == CERA_TYPE_F16) return q_type == type ? go(__half(), __half()) : go(__half(), float());
+    return q_type == type ? go(__nv_bfloat16(), __nv_bfloat16()) : go(__nv_bfloat16(), float());
+}
+
+}  // namespace cera

@@ -129,6 +129,14 @@ __device__ __forceinline__ void tensor_g2s_2d_if(void *dst, const void *map, int
         "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(me)
         : "memory");
 }
+// One box of a tensor map of four dimensions.  x * element size is a multiple of 16 bytes.
+__device__ __forceinline__ void tensor_g2s_4d_if(void *dst, const void *map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t *bar, uint32_t me) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(me)
+        : "memory");
+}
 // Its bytes counted on a barrier (cluster address) of this CTA or its cta_group::2 peer.
 __device__ __forceinline__ void tensor_g2s_2d_pair_if(void *dst, const void *map, int32_t x, int32_t y, uint32_t bar, uint32_t me) {
     asm volatile(
