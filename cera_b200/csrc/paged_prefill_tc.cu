@@ -58,7 +58,7 @@ struct Pp {
     static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
     static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
     static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((NP * P_COLS > KT ? NP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
-    static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 3);
+    static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 4);  // warpgroups: softmax of a tile each; products, two loaders and a warp of nothing
     static constexpr size_t SMEM = 1024 + (size_t)MT * NP * QPART + (size_t)ST * 2 * HALF;
     static_assert(ST >= 1 && MT * T_COLS <= 512, "does not fit");
 };
@@ -70,6 +70,11 @@ struct PpBars {
 __device__ __forceinline__ float pp_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pp_max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -135,6 +140,8 @@ struct PpWork {
     int32_t p0;                       // the slot of its first token, negative if it has none
     PagedSpan span;
     uint32_t x0, x1;
+    int32_t lo[2], hi[2];   // per tile of rows: the slots of its first and last row, and what the first's window begins with
+    uint32_t first[2];
 
     __device__ __forceinline__ int32_t slot_of(uint32_t row, uint32_t group) const { return p0 + (int32_t)(row / group); }
 };
@@ -182,19 +189,21 @@ __device__ __forceinline__ void pp_set(const PpParams &p, PpWork &w) {
     const uint32_t last = min(w.row0 + C::MT * PP_ROWS, w.rows) - 1;
     const int32_t lo = max(w.slot_of(w.row0, p.group), 0), hi = w.slot_of(last, p.group) + 1;
     w.span.set(p.mask, (uint32_t)lo, (uint32_t)max(hi, 0), C::KT);
+    for (uint32_t t = 0; t < 2; ++t) {
+        const uint32_t a = w.row0 + t * PP_ROWS;
+        const bool some = t < C::MT && a < w.rows;
+        w.lo[t] = some ? w.slot_of(a, p.group) : -1;
+        w.hi[t] = some ? w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group) : -1;
+        w.first[t] = paged_first(p.mask, (uint32_t)max(w.lo[t], 0));
+    }
     w.x0 = (uint32_t)((uint64_t)w.span.tiles * blockIdx.z / gridDim.z);
     w.x1 = (uint32_t)((uint64_t)w.span.tiles * (blockIdx.z + 1) / gridDim.z);
 }
 
 // Whether tile t of the CTA's rows sees something of the key tile at slot0.
-template <int DP, int NP>
+template <int KT>
 __device__ __forceinline__ bool pp_sees(const PpParams &p, const PpWork &w, uint32_t t, uint32_t slot0) {
-    const uint32_t a = w.row0 + t * PP_ROWS;
-    if (a >= w.rows) return false;
-    const int32_t hi = w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group);
-    if (hi < (int32_t)slot0) return false;
-    const uint32_t first = paged_first(p.mask, (uint32_t)max(w.slot_of(a, p.group), 0));
-    return slot0 + Pp<DP, NP>::KT > first || slot0 < p.mask.sink;
+    return w.hi[t] >= (int32_t)slot0 && (slot0 + KT > w.first[t] || slot0 < p.mask.sink);
 }
 
 // The keys' or the values' loader, a warp.
@@ -300,14 +309,14 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
     if (n == 0 || !arrived(&b->q_full, 0) || !arrived(&b->k_full[0], 0)) return;
     tc_fence_after();
     for (uint32_t t = 0; t < C::MT; ++t)
-        if (pp_sees<DP, NP>(p, w, t, slot0(0))) score(t, 0);
+        if (pp_sees<C::KT>(p, w, t, slot0(0))) score(t, 0);
     tc_commit(&b->k_empty[0], me);
     for (uint32_t i = 0; i < n; ++i) {
         const uint32_t st = i % C::ST, next = (i + 1) % C::ST;
         bool there = false, ready = false;
         uint8_t *vt = vs + st * C::HALF;
         for (uint32_t t = 0; t < C::MT; ++t) {
-            if (pp_sees<DP, NP>(p, w, t, slot0(i))) {
+            if (pp_sees<C::KT>(p, w, t, slot0(i))) {
                 if (!arrived(&b->p_full[t], added[t] & 1)) return;
                 if (!there) {
                     if (!arrived(&b->v_full[st], i / C::ST & 1)) return;
@@ -336,7 +345,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
                         tc_mma_f16_ts(o, tmem + t * C::T_COLS + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
                 ++added[t];
             }
-            if (i + 1 < n && pp_sees<DP, NP>(p, w, t, slot0(i + 1))) {
+            if (i + 1 < n && pp_sees<C::KT>(p, w, t, slot0(i + 1))) {
                 if (!ready) {
                     if (!arrived(&b->k_full[next], (i + 1) / C::ST & 1)) return;
                     tc_fence_after();
@@ -409,7 +418,6 @@ template <typename T, typename TQ, int DP, int NP>
 __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, uint32_t t, uint8_t *qs, uint32_t tmem, PpBars *b, const uint32_t (*masks)[4],
                                            volatile uint32_t *abort_flag, unsigned int *status) {
     using C = Pp<DP, NP>;
-    constexpr int CH = NP == 1 ? 32 : C::KT;  // columns taken at a time: P goes over columns of S that have been read
     const uint32_t lane = threadIdx.x & 31, quad = threadIdx.x >> 5 & 3, r = quad * 32 + lane, row = w.row0 + t * PP_ROWS + r;
     const uint32_t ts = tmem + t * C::T_COLS + (quad * 32 << 16), to = ts + C::S_COLS;
     const float c = pp_queries<T, TQ, DP, NP>(p, w, row, qs + t * NP * C::QPART, r);
@@ -417,10 +425,10 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     __syncwarp();
     if (lane == 0) tma::mbar_arrive(&b->q_full);
 
-    const uint32_t a = w.row0 + t * PP_ROWS, z = min(a + PP_ROWS, w.rows);
+    const uint32_t a = w.row0 + t * PP_ROWS;
     const bool live = row < w.rows;
     const int32_t pos = live ? w.slot_of(row, p.group) : -1;
-    const int32_t p_lo = a < w.rows ? w.slot_of(a, p.group) : -1, p_hi = a < w.rows ? w.slot_of(z - 1, p.group) : -1;
+    const int32_t p_lo = w.lo[t], p_hi = w.hi[t];
     const int32_t first = pos >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)pos) : 0, first_hi = p_hi >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)p_hi) : 0;
     const int32_t sinks = (int32_t)min(p.mask.sink, (uint32_t)max(first, 0));
     float m = PP_FLOOR, l = 0.0f;
@@ -428,7 +436,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     bool ok = true;
     for (uint32_t i = 0; i < w.x1 - w.x0; ++i) {
         const uint32_t slot0 = w.span.slot(w.x0 + i, C::KT);
-        if (!pp_sees<DP, NP>(p, w, t, slot0)) continue;
+        if (!pp_sees<C::KT>(p, w, t, slot0)) continue;
         ok = tma::mbar_wait_warp(&b->s_full[t], done & 1, abort_flag, status, 4u);
         if (!ok) break;
         tc_fence_after();
@@ -447,23 +455,25 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 see[k] &= pp_low(pos + 1 - at) & (~pp_low(first - at) | pp_low(sinks - at));
             }
         }
-        float mx = -INFINITY;
-        uint32_t v[CH / 32][32];
+        // the tile's scores at once, their largest in four chains
+        uint32_t v[C::KT / 32][32];
 #pragma unroll
-        for (int k = 0; k < C::KT / CH; ++k) {
+        for (int j = 0; j < C::KT / 32; ++j) tmem_ld32(ts + 32 * j, v[j]);
+        tmem_wait_ld();
+        if (!all) {
 #pragma unroll
-            for (int j = 0; j < CH / 32; ++j) tmem_ld32(ts + k * CH + 32 * j, v[j]);
-            tmem_wait_ld();
+            for (int j = 0; j < C::KT / 32; ++j)
 #pragma unroll
-            for (int j = 0; j < CH / 32; ++j) {
-                if (!all) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[j][e] = see[k * (CH / 32) + j] >> e & 1 ? v[j][e] : 0xff800000u;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[j][e]));
-            }
+                for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
         }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < C::KT / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
+        float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         mx *= c;
         float f = 1.0f;
         if (mx > m + PP_RAISE) {
@@ -482,36 +492,25 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 tmem_st16(to + d + 16, *reinterpret_cast<const uint32_t(*)[16]>(o + 16));
             }
         }
-        const float base = PP_LIFT - m;
+        const float2 base = make_float2(PP_LIFT - m, PP_LIFT - m), cc = make_float2(c, c);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-        for (int k = 0; k < C::KT / CH; ++k) {
-            if (C::KT > CH) {  // not in registers any more
+        for (int j = 0; j < C::KT / 32; ++j) {
+            uint32_t wd[NP][16];
 #pragma unroll
-                for (int j = 0; j < CH / 32; ++j) tmem_ld32(ts + k * CH + 32 * j, v[j]);
-                tmem_wait_ld();
-                if (!all) {
+            for (int e = 0; e < 16; ++e) {
+                float2 x = __ffma2_rn(make_float2(__uint_as_float(v[j][2 * e]), __uint_as_float(v[j][2 * e + 1])), cc, base);
+                x = make_float2(pp_exp2(x.x), pp_exp2(x.y));
+                sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+                uint32_t u[NP];
+                pp_parts<T, NP>(x.x, x.y, u);
 #pragma unroll
-                    for (int j = 0; j < CH / 32; ++j)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[j][e] = see[k * (CH / 32) + j] >> e & 1 ? v[j][e] : 0xff800000u;
-                }
+                for (int n = 0; n < NP; ++n) wd[n][e] = u[n];
             }
 #pragma unroll
-            for (int j = 0; j < CH / 32; ++j) {
-                uint32_t wd[NP][16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = pp_exp2(fmaf(__uint_as_float(v[j][2 * e]), c, base)), y = pp_exp2(fmaf(__uint_as_float(v[j][2 * e + 1]), c, base));
-                    l += x + y;
-                    uint32_t u[NP];
-                    pp_parts<T, NP>(x, y, u);
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) wd[n][e] = u[n];
-                }
-#pragma unroll
-                for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + k * (CH / 2) + 16 * j, wd[n]);
-            }
+            for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + 16 * j, wd[n]);
         }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -617,12 +616,17 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     const uint32_t tmem = tmem_at;
     unsigned int *status = &g_paged_prefill_status;
     if (warp < C::MATH) {
+        if (C::MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // of 168 x 384 at the launch: 208 x 256 + 80 x 128 are 1024 less
         pp_softmax<T, TQ, DP, NP>(p, w, warp / 4, qs, tmem, &bars, masks, &abort_s, status);
-    } else if (warp == C::MATH) {
-        pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, masks, &abort_s, status);
     } else {
-        const bool is_v = warp == C::MATH + 2;
-        pp_load<T, DP, NP, TMA>(p, w, is_v ? &map_v : &map_k, is_v, is_v ? vs : ks, is_v ? bars.v_full : bars.k_full, is_v ? bars.v_empty : bars.k_empty, masks, &abort_s, status);
+        if (C::MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == C::MATH) {
+            pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, masks, &abort_s, status);
+        } else if (warp < C::MATH + 3) {
+            const bool is_v = warp == C::MATH + 2;
+            pp_load<T, DP, NP, TMA>(p, w, is_v ? &map_v : &map_k, is_v, is_v ? vs : ks, is_v ? bars.v_full : bars.k_full, is_v ? bars.v_empty : bars.k_empty, masks, &abort_s,
+                                    status);
+        }
     }
     __syncwarp();
     tc_fence_before();
