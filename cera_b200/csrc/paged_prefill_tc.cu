@@ -54,7 +54,6 @@ template <int DP, int NP>
 struct Pp {
     static constexpr int MT = DP <= 128 ? 2 : 1;
     static constexpr int KT = NP == 1 ? 128 : DP == 256 && NP == 3 ? 32 : 64;
-    static constexpr int BLOCKS = DP / 64;
     static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
     static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
     static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((NP * P_COLS > KT ? NP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
@@ -64,7 +63,7 @@ struct Pp {
 };
 
 struct PpBars {
-    uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, v_part, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], o_full[2];
 };
 
 __device__ __forceinline__ float pp_exp2(float x) {
@@ -85,6 +84,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr)
         : "memory");
+}
+// Waits for every load so far; what follows uses these registers.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 // D (+)= A[tmem] * B[smem], kind::f16.
 __device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t me) {
@@ -209,7 +220,7 @@ __device__ __forceinline__ bool pp_sees(const PpParams &p, const PpWork &w, uint
 // The keys' or the values' loader, a warp.
 template <typename T, int DP, int NP, bool TMA>
 __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, const CUtensorMap *map, bool is_v, uint8_t *stages, uint64_t *full, uint64_t *empty,
-                                        uint32_t (*masks)[4], volatile uint32_t *abort_flag, unsigned int *status) {
+                                        uint64_t *part, uint32_t (*masks)[4], volatile uint32_t *abort_flag, unsigned int *status) {
     using C = Pp<DP, NP>;
     const uint32_t lane = threadIdx.x & 31, h = blockIdx.y, boxes = C::KT / p.box, blocks = (p.kv.dim + 63) / 64, me = elect_one();
     const size_t by_page = is_v ? p.kv.v_page : p.kv.k_page, by_slot = is_v ? p.kv.v_slot : p.kv.k_slot, by_head = is_v ? p.kv.v_head : p.kv.k_head;
@@ -232,6 +243,13 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
             }
         }
     };
+    uint32_t parts = 0;
+    // given up: shared memory must outlive the copies in flight, those of the stages before tile n and, if the last was not whole, its own
+    auto drain = [&](uint32_t n, bool all) {
+        for (uint32_t y = n > C::ST ? n - C::ST : 0; y < n; ++y)
+            for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % C::ST], y / C::ST & 1); ++i) __nanosleep(40);
+        for (uint32_t i = 0; !all && i < tma::SPIN_LIMIT && !tma::mbar_test(part, (parts - 1) & 1); ++i) __nanosleep(40);
+    };
     if (w.x0 < w.x1) find(w.x0);
     for (uint32_t x = w.x0; x < w.x1; ++x) {
         const uint32_t i0 = x - w.x0, st = i0 % C::ST, slot0 = w.span.slot(x, C::KT);
@@ -245,11 +263,7 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
             mask[i] = __ballot_sync(0xffffffffu, TMA ? w.span.sees(slot0 + j) && (live >> j / p.box & 1) : pg[i] != NO_PAGE);
         }
         if (x + 1 < w.x1) find(x + 1);  // its answer is not needed before the next tile
-        if (!tma::mbar_wait_warp(&empty[st], (i0 / C::ST & 1) ^ 1, abort_flag, status, 1u)) {  // given up: shared memory must outlive the copies in flight
-            for (uint32_t y = i0 > C::ST ? i0 - C::ST : 0; y < i0; ++y)
-                for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % C::ST], y / C::ST & 1); ++i) __nanosleep(40);
-            return;
-        }
+        if (!tma::mbar_wait_warp(&empty[st], (i0 / C::ST & 1) ^ 1, abort_flag, status, 1u)) return drain(i0, true);
         if (!is_v) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -257,12 +271,34 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
         }
         __syncwarp();
         uint8_t *to = stages + st * C::HALF;
+        // rows of values that are not seen are set to zero when the rest is there: a weight of zero times what lies there could be a NaN
+        bool whole = !is_v;
+        if (is_v) {
+            whole = true;
+#pragma unroll
+            for (int i = 0; i < N; ++i) whole = whole && mask[i] == 0xffffffffu;
+        }
+        auto clear = [&]() {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (mask[i] >> lane & 1) continue;
+                for (uint32_t c = 0; c < blocks * 8; ++c) *reinterpret_cast<uint4 *>(to + (c >> 3) * C::KBLOCK + (32 * i + lane) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+        };
         if (TMA) {
-            tma::mbar_expect_tx_if(&full[st], __popc(live) * blocks * p.box * 128, me);
+            uint64_t *bar = whole ? &full[st] : part;
+            tma::mbar_expect_tx_if(bar, __popc(live) * blocks * p.box * 128, me);
             for (uint32_t i = 0; i < boxes; ++i) {
                 const uint32_t pi = __shfl_sync(0xffffffffu, pg[0], i), ri = __shfl_sync(0xffffffffu, rw[0], i);
                 if (pi == NO_PAGE) continue;
-                for (uint32_t k = 0; k < blocks; ++k) tma::tensor_g2s_4d_if(to + k * C::KBLOCK + i * p.box * 128, map, k * 64, h, ri, pi, &full[st], me);
+                for (uint32_t k = 0; k < blocks; ++k) tma::tensor_g2s_4d_if(to + k * C::KBLOCK + i * p.box * 128, map, k * 64, h, ri, pi, bar, me);
+            }
+            if (!whole) {
+                if (!tma::mbar_wait_warp(part, parts++ & 1, abort_flag, status, 1u)) return drain(i0, false);
+                clear();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tma::mbar_arrive(&full[st]);
             }
         } else {
             const uint32_t per = blocks * 8, used = p.kv.dim / 8;
@@ -277,6 +313,7 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
             }
             // what these copies write is read by the tensor cores: complete, fenced, then announced
             asm volatile("cp.async.wait_all;" ::: "memory");
+            if (!whole) clear();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) tma::mbar_arrive(&full[st]);
@@ -284,84 +321,74 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
     }
 }
 
-// The products, a warp.
+// The products, a warp that stays together (descriptors live in registers that a warp has once: a branch of one lane around them mixes them up): of each tile of rows
+// in turn O += P V of these keys, then S of the next.
 template <typename T, int DP, int NP>
-__device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, uint8_t *qs, uint8_t *ks, uint8_t *vs, uint32_t tmem, PpBars *b, const uint32_t (*masks)[4],
-                                            volatile uint32_t *abort_flag, unsigned int *status) {
+__device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, uint8_t *qs, uint8_t *ks, uint8_t *vs, uint32_t tmem, PpBars *b, volatile uint32_t *abort_flag,
+                                            unsigned int *status) {
     using C = Pp<DP, NP>;
     constexpr bool BF = !std::is_same<T, __half>::value;
-    const uint32_t lane = threadIdx.x & 31, me = elect_one(), id_s = pp_idesc(BF, C::KT, false), id_o = pp_idesc(BF, p.kv.dim, true), n = w.x1 - w.x0;
+    const uint32_t me = elect_one(), id_s = pp_idesc(BF, C::KT, false), id_o = pp_idesc(BF, p.kv.dim, true), n = w.x1 - w.x0, steps = p.kv.dim / 16;
+    const uint64_t q0 = smem_desc_sw128(tma::smem_u32(qs)), k0 = smem_desc_sw128(tma::smem_u32(ks)), v0 = pp_desc_v(tma::smem_u32(vs), C::KBLOCK);  // address fields count 16 bytes
     auto arrived = [&](uint64_t *bar, uint32_t parity) { return tma::mbar_wait_warp(bar, parity, abort_flag, status, 2u); };
-    auto slot0 = [&](uint32_t i) { return w.span.slot(w.x0 + i, C::KT); };
-    uint32_t scored[2] = {0, 0}, added[2] = {0, 0};
-    auto score = [&](uint32_t t, uint32_t i) {
+    uint32_t added[2] = {0, 0};
+    auto score = [&](uint32_t t, uint32_t st) {
         const uint32_t d = tmem + t * C::T_COLS;
-        const uint64_t kd = smem_desc_sw128(tma::smem_u32(ks + i % C::ST * C::HALF));
-        uint32_t acc = 0;
+        const uint64_t kd = k0 + st * (C::HALF / 16);
+#pragma unroll 1
         for (int part = 0; part < NP; ++part) {
-            const uint64_t qd = smem_desc_sw128(tma::smem_u32(qs + (t * NP + part) * C::QPART));
-            for (uint32_t k = 0; k < p.kv.dim / 16; ++k, acc = 1)
-                tc_mma_f16(d, qd + (k >> 2) * (C::QBLOCK / 16) + 2 * (k & 3), kd + (k >> 2) * (C::KBLOCK / 16) + 2 * (k & 3), id_s, acc, me);
+            const uint64_t qd = q0 + (t * NP + part) * (C::QPART / 16);
+#pragma unroll
+            for (uint32_t k = 0; k < DP / 16; ++k)
+                if (k < steps) tc_mma_f16(d, qd + (k >> 2) * (C::QBLOCK / 16) + 2 * (k & 3), kd + (k >> 2) * (C::KBLOCK / 16) + 2 * (k & 3), id_s, part | k, me);
         }
         tc_commit(&b->s_full[t], me);
-        ++scored[t];
     };
     if (n == 0 || !arrived(&b->q_full, 0) || !arrived(&b->k_full[0], 0)) return;
     tc_fence_after();
-    for (uint32_t t = 0; t < C::MT; ++t)
-        if (pp_sees<C::KT>(p, w, t, slot0(0))) score(t, 0);
-    tc_commit(&b->k_empty[0], me);
-    for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t st = i % C::ST, next = (i + 1) % C::ST;
-        bool there = false, ready = false;
-        uint8_t *vt = vs + st * C::HALF;
-        for (uint32_t t = 0; t < C::MT; ++t) {
-            if (pp_sees<C::KT>(p, w, t, slot0(i))) {
-                if (!arrived(&b->p_full[t], added[t] & 1)) return;
-                if (!there) {
-                    if (!arrived(&b->v_full[st], i / C::ST & 1)) return;
-                    there = true;
-                    // rows that were not loaded: a weight of zero times what lies there could be a NaN
-                    bool fixed = false;
+    uint32_t slot = w.span.slot(w.x0, C::KT);
 #pragma unroll
-                    for (int m = 0; m < (C::KT + 31) / 32; ++m) {
-                        const uint32_t mask = masks[i % PP_MASKS][m];
-                        if (mask == 0xffffffffu) continue;
-                        fixed = true;
-                        for (uint32_t r = 0; r < 32; ++r)
-                            if (!(mask >> r & 1))
-                                for (uint32_t c = lane; c < DP / 8; c += 32) *reinterpret_cast<uint4 *>(vt + (c >> 3) * C::KBLOCK + (32 * m + r) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    if (fixed) {
-                        fence_async_smem();
-                        __syncwarp();
-                    }
-                }
+    for (uint32_t t = 0; t < C::MT; ++t)
+        if (pp_sees<C::KT>(p, w, t, slot)) score(t, 0);
+    tc_commit(&b->k_empty[0], me);
+    uint32_t st = 0, turn = 0;  // the stage of these keys and how often the ring has gone round
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint32_t next = st + 1 == C::ST ? 0 : st + 1, next_turn = st + 1 == C::ST ? turn ^ 1 : turn, slot_next = i + 1 < n ? w.span.slot(w.x0 + i + 1, C::KT) : 0;
+        bool there = false, ready = false;
+#pragma unroll
+        for (uint32_t t = 0; t < C::MT; ++t) {
+            if (pp_sees<C::KT>(p, w, t, slot)) {
+                if (!there && !arrived(&b->v_full[st], turn)) return;
+                there = true;
+                if (!arrived(&b->p_full[t], added[t] & 1)) return;
                 tc_fence_after();
-                const uint32_t o = tmem + t * C::T_COLS + C::S_COLS;
-                const uint64_t vd = pp_desc_v(tma::smem_u32(vt), C::KBLOCK);
+                const uint32_t s = tmem + t * C::T_COLS, o = s + C::S_COLS;
+                const uint64_t vd = v0 + st * (C::HALF / 16);
+#pragma unroll 1
                 for (int part = 0; part < NP; ++part)
-                    for (uint32_t k = 0; k < C::KT / 16; ++k)
-                        tc_mma_f16_ts(o, tmem + t * C::T_COLS + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
+#pragma unroll
+                    for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
                 ++added[t];
             }
-            if (i + 1 < n && pp_sees<C::KT>(p, w, t, slot0(i + 1))) {
-                if (!ready) {
-                    if (!arrived(&b->k_full[next], (i + 1) / C::ST & 1)) return;
-                    tc_fence_after();
-                    ready = true;
-                }
-                score(t, i + 1);
+            if (i + 1 < n && pp_sees<C::KT>(p, w, t, slot_next)) {
+                if (!ready && !arrived(&b->k_full[next], next_turn)) return;
+                ready = true;
+                tc_fence_after();
+                score(t, next);
             }
         }
         // a stage that no tile of rows saw has to have arrived before it is filled again
-        if (!there && !arrived(&b->v_full[st], i / C::ST & 1)) return;
+        if (!there && !arrived(&b->v_full[st], turn)) return;
         tc_commit(&b->v_empty[st], me);
         if (i + 1 < n) {
-            if (!ready && !arrived(&b->k_full[next], (i + 1) / C::ST & 1)) return;
+            if (!ready && !arrived(&b->k_full[next], next_turn)) return;
             tc_commit(&b->k_empty[next], me);
         }
+        st = next;
+        turn = next_turn;
+        slot = slot_next;
     }
+#pragma unroll
     for (uint32_t t = 0; t < C::MT; ++t) tc_commit(&b->o_full[t], me);
 }
 
@@ -455,47 +482,18 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 see[k] &= pp_low(pos + 1 - at) & (~pp_low(first - at) | pp_low(sinks - at));
             }
         }
-        // the tile's scores at once, their largest in four chains
-        uint32_t v[C::KT / 32][32];
+        // Weights for the maximum that is known, a quarter of the tile's scores while the next comes from TMEM; where the tile has a score past it by more than 2^8, O and the
+        // sum are rescaled and the weights, whose scores are still in registers, formed again.
+        constexpr int Q = C::KT / 32;
+        uint32_t v[Q][32];
+        tmem_ld32(ts, v[0]);
+        if (NP > 1) {  // the parts of P lie where scores are
 #pragma unroll
-        for (int j = 0; j < C::KT / 32; ++j) tmem_ld32(ts + 32 * j, v[j]);
-        tmem_wait_ld();
-        if (!all) {
-#pragma unroll
-            for (int j = 0; j < C::KT / 32; ++j)
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
+            for (int j = 1; j < Q; ++j) tmem_ld32(ts + 32 * j, v[j]);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < C::KT / 32; ++j)
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
-        float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        mx *= c;
-        float f = 1.0f;
-        if (mx > m + PP_RAISE) {
-            f = pp_exp2(m - mx);
-            m = mx;
-            l *= f;
-        }
-        if (done && __any_sync(0xffffffffu, f != 1.0f)) {  // O is complete up to the tile before, and nothing adds to it
-            for (uint32_t d = 0; d < p.kv.dim; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + d, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st16(to + d, *reinterpret_cast<const uint32_t(*)[16]>(o));
-                tmem_st16(to + d + 16, *reinterpret_cast<const uint32_t(*)[16]>(o + 16));
-            }
-        }
-        const float2 base = make_float2(PP_LIFT - m, PP_LIFT - m), cc = make_float2(c, c);
-        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-        for (int j = 0; j < C::KT / 32; ++j) {
+        float2 base = make_float2(PP_LIFT - m, PP_LIFT - m), sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 cc = make_float2(c, c);
+        auto form = [&](int j) {
             uint32_t wd[NP][16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -509,6 +507,40 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             }
 #pragma unroll
             for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + 16 * j, wd[n]);
+        };
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+            tmem_wait_ld32(v[j]);
+            if (NP == 1 && j + 1 < Q) tmem_ld32(ts + 32 * (j + 1), v[j + 1 < Q ? j + 1 : j]);
+            if (!all) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
+            form(j);
+        }
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const bool raise = mx > m + PP_RAISE;
+        if (__any_sync(0xffffffffu, raise)) {
+            const float f = raise ? pp_exp2(m - mx) : 1.0f;
+            if (raise) m = mx;
+            l *= f;
+            for (uint32_t d = 0; done && d < p.kv.dim; d += 16) {  // O is complete up to the tile before, and nothing adds to it
+                uint32_t o[16];
+                tmem_ld16(to + d, o);
+                tmem_wait_ld16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(to + d, o);
+            }
+            base = make_float2(PP_LIFT - m, PP_LIFT - m);
+            sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < Q; ++j) form(j);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
@@ -528,7 +560,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             for (uint32_t d = 0; d < p.kv.dim; d += 32) {
                 uint32_t o[32];
                 tmem_ld32(to + d, o);
-                tmem_wait_ld();
+                tmem_wait_ld32(o);
                 if (live) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(p.part + at * p.kv.dim + d + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -543,7 +575,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
         uint32_t o[32];
         if (done) {
             tmem_ld32(to + d, o);
-            tmem_wait_ld();
+            tmem_wait_ld32(o);
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 16 / sizeof(TQ)) {
@@ -588,6 +620,7 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
             work = w;
             abort_s = 0;
             tma::mbar_init(&bars.q_full, C::MATH);
+            tma::mbar_init(&bars.v_part, 1);
             for (int i = 0; i < 3; ++i) {
                 tma::mbar_init(&bars.k_full[i], 1);
                 tma::mbar_init(&bars.v_full[i], 1);
@@ -621,10 +654,10 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     } else {
         if (C::MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == C::MATH) {
-            pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, masks, &abort_s, status);
+            pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, &abort_s, status);
         } else if (warp < C::MATH + 3) {
             const bool is_v = warp == C::MATH + 2;
-            pp_load<T, DP, NP, TMA>(p, w, is_v ? &map_v : &map_k, is_v, is_v ? vs : ks, is_v ? bars.v_full : bars.k_full, is_v ? bars.v_empty : bars.k_empty, masks, &abort_s,
+            pp_load<T, DP, NP, TMA>(p, w, is_v ? &map_v : &map_k, is_v, is_v ? vs : ks, is_v ? bars.v_full : bars.k_full, is_v ? bars.v_empty : bars.k_empty, &bars.v_part, masks, &abort_s,
                                     status);
         }
     }
