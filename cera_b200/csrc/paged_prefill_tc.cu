@@ -151,8 +151,8 @@ struct PpWork {
     int32_t p0;                       // the slot of its first token, negative if it has none
     PagedSpan span;
     uint32_t x0, x1;
-    int32_t lo[2], hi[2];   // per tile of rows: the slots of its first and last row, and what the first's window begins with
-    uint32_t first[2];
+    int32_t lo0, lo1, hi0, hi1;  // of either tile of rows: the slots of its first and last row, and what the first's window begins with
+    uint32_t first0, first1;
 
     __device__ __forceinline__ int32_t slot_of(uint32_t row, uint32_t group) const { return p0 + (int32_t)(row / group); }
 };
@@ -198,15 +198,16 @@ __device__ __forceinline__ void pp_set(const PpParams &p, PpWork &w) {
     w.len = paged_len(p.kv, w.s);
     w.p0 = (int32_t)w.len - (int32_t)(w.rows / p.group);
     const uint32_t last = min(w.row0 + C::MT * PP_ROWS, w.rows) - 1;
-    const int32_t lo = max(w.slot_of(w.row0, p.group), 0), hi = w.slot_of(last, p.group) + 1;
-    w.span.set(p.mask, (uint32_t)lo, (uint32_t)max(hi, 0), C::KT);
-    for (uint32_t t = 0; t < 2; ++t) {
+    w.span.set(p.mask, (uint32_t)max(w.slot_of(w.row0, p.group), 0), (uint32_t)max(w.slot_of(last, p.group) + 1, 0), C::KT);
+    auto tile = [&](uint32_t t, int32_t &lo, int32_t &hi, uint32_t &first) {
         const uint32_t a = w.row0 + t * PP_ROWS;
         const bool some = t < C::MT && a < w.rows;
-        w.lo[t] = some ? w.slot_of(a, p.group) : -1;
-        w.hi[t] = some ? w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group) : -1;
-        w.first[t] = paged_first(p.mask, (uint32_t)max(w.lo[t], 0));
-    }
+        lo = some ? w.slot_of(a, p.group) : -1;
+        hi = some ? w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group) : -1;
+        first = paged_first(p.mask, (uint32_t)max(lo, 0));
+    };
+    tile(0, w.lo0, w.hi0, w.first0);
+    tile(1, w.lo1, w.hi1, w.first1);
     w.x0 = (uint32_t)((uint64_t)w.span.tiles * blockIdx.z / gridDim.z);
     w.x1 = (uint32_t)((uint64_t)w.span.tiles * (blockIdx.z + 1) / gridDim.z);
 }
@@ -214,7 +215,7 @@ __device__ __forceinline__ void pp_set(const PpParams &p, PpWork &w) {
 // Whether tile t of the CTA's rows sees something of the key tile at slot0.
 template <int KT>
 __device__ __forceinline__ bool pp_sees(const PpParams &p, const PpWork &w, uint32_t t, uint32_t slot0) {
-    return w.hi[t] >= (int32_t)slot0 && (slot0 + KT > w.first[t] || slot0 < p.mask.sink);
+    return (t ? w.hi1 : w.hi0) >= (int32_t)slot0 && (slot0 + KT > (t ? w.first1 : w.first0) || slot0 < p.mask.sink);
 }
 
 // The keys' or the values' loader, a warp.
@@ -455,7 +456,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     const uint32_t a = w.row0 + t * PP_ROWS;
     const bool live = row < w.rows;
     const int32_t pos = live ? w.slot_of(row, p.group) : -1;
-    const int32_t p_lo = w.lo[t], p_hi = w.hi[t];
+    const int32_t p_lo = t ? w.lo1 : w.lo0, p_hi = t ? w.hi1 : w.hi0;
     const int32_t first = pos >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)pos) : 0, first_hi = p_hi >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)p_hi) : 0;
     const int32_t sinks = (int32_t)min(p.mask.sink, (uint32_t)max(first, 0));
     float m = PP_FLOOR, l = 0.0f;
@@ -509,20 +510,24 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + 16 * j, wd[n]);
         };
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto stream = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < Q; ++j) {
-            tmem_wait_ld32(v[j]);
-            if (NP == 1 && j + 1 < Q) tmem_ld32(ts + 32 * (j + 1), v[j + 1 < Q ? j + 1 : j]);
-            if (!all) {
+            for (int j = 0; j < Q; ++j) {
+                tmem_wait_ld32(v[j]);
+                if (NP == 1 && j + 1 < Q) tmem_ld32(ts + 32 * (j + 1), v[j + 1 < Q ? j + 1 : j]);
+                if (!decltype(whole)::value) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
+                    for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
+                form(j);
             }
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
-            form(j);
-        }
+        };
+        if (all) stream(std::true_type());
+        else stream(std::false_type());
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
         const bool raise = mx > m + PP_RAISE;
         if (__any_sync(0xffffffffu, raise)) {
@@ -555,7 +560,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     const size_t place = ((size_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group);
     if (gridDim.z > 1) {
         const size_t at = (size_t)blockIdx.z * p.n * p.heads + place;
-        if (live) p.ml[at] = make_float2(l > 0.0f || l != l || m != PP_FLOOR ? m : -INFINITY, l);
+        if (live) p.ml[at] = make_float2(l != l || m != PP_FLOOR ? m : -INFINITY, l);
         if (done)
             for (uint32_t d = 0; d < p.kv.dim; d += 32) {
                 uint32_t o[32];
@@ -570,7 +575,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     }
     TQ *out = reinterpret_cast<TQ *>(p.out) + place * p.kv.dim;
     const float f = 1.0f / l;
-    float check = l > 0.0f ? 0.0f : NAN;
+    float check = l > 0.0f && m != PP_FLOOR ? 0.0f : NAN;
     for (uint32_t d = 0; d < p.kv.dim; d += 32) {
         uint32_t o[32];
         if (done) {
