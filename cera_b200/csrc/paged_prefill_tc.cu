@@ -348,19 +348,28 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
     if (n == 0 || !arrived(&b->q_full, 0) || !arrived(&b->k_full[0], 0)) return;
     tc_fence_after();
     uint32_t slot = w.span.slot(w.x0, C::KT);
+    bool sees[2] = {pp_sees<C::KT>(p, w, 0, slot), C::MT == 2 && pp_sees<C::KT>(p, w, 1, slot)};
 #pragma unroll
     for (uint32_t t = 0; t < C::MT; ++t)
-        if (pp_sees<C::KT>(p, w, t, slot)) score(t, 0);
+        if (sees[t]) score(t, 0);
     tc_commit(&b->k_empty[0], me);
     uint32_t st = 0, turn = 0;  // the stage of these keys and how often the ring has gone round
     for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t next = st + 1 == C::ST ? 0 : st + 1, next_turn = st + 1 == C::ST ? turn ^ 1 : turn, slot_next = i + 1 < n ? w.span.slot(w.x0 + i + 1, C::KT) : 0;
-        bool there = false, ready = false;
+        const bool more = i + 1 < n;
+        const uint32_t next = st + 1 == C::ST ? 0 : st + 1, next_turn = st + 1 == C::ST ? turn ^ 1 : turn;
+        bool then[2] = {false, false};
+        // what was loaded is waited for ahead of the weights, which are what is waited for in earnest; a stage that no tile of rows sees has to have arrived too
+        // before it is filled again
+        if (more) {
+            slot = w.span.slot(w.x0 + i + 1, C::KT);
+            then[0] = pp_sees<C::KT>(p, w, 0, slot);
+            then[1] = C::MT == 2 && pp_sees<C::KT>(p, w, 1, slot);
+            if (!arrived(&b->k_full[next], next_turn)) return;
+        }
+        if (!arrived(&b->v_full[st], turn)) return;
 #pragma unroll
         for (uint32_t t = 0; t < C::MT; ++t) {
-            if (pp_sees<C::KT>(p, w, t, slot)) {
-                if (!there && !arrived(&b->v_full[st], turn)) return;
-                there = true;
+            if (sees[t]) {
                 if (!arrived(&b->p_full[t], added[t] & 1)) return;
                 tc_fence_after();
                 const uint32_t s = tmem + t * C::T_COLS, o = s + C::S_COLS;
@@ -371,23 +380,14 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
                     for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
                 ++added[t];
             }
-            if (i + 1 < n && pp_sees<C::KT>(p, w, t, slot_next)) {
-                if (!ready && !arrived(&b->k_full[next], next_turn)) return;
-                ready = true;
-                tc_fence_after();
-                score(t, next);
-            }
+            if (t + 1 == C::MT) tc_commit(&b->v_empty[st], me);
+            if (then[t]) score(t, next);
         }
-        // a stage that no tile of rows saw has to have arrived before it is filled again
-        if (!there && !arrived(&b->v_full[st], turn)) return;
-        tc_commit(&b->v_empty[st], me);
-        if (i + 1 < n) {
-            if (!ready && !arrived(&b->k_full[next], next_turn)) return;
-            tc_commit(&b->k_empty[next], me);
-        }
+        if (more) tc_commit(&b->k_empty[next], me);
         st = next;
         turn = next_turn;
-        slot = slot_next;
+        sees[0] = then[0];
+        sees[1] = then[1];
     }
 #pragma unroll
     for (uint32_t t = 0; t < C::MT; ++t) tc_commit(&b->o_full[t], me);
@@ -483,15 +483,14 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 see[k] &= pp_low(pos + 1 - at) & (~pp_low(first - at) | pp_low(sinks - at));
             }
         }
-        // Weights for the maximum that is known, a quarter of the tile's scores while the next comes from TMEM; where the tile has a score past it by more than 2^8, O and the
+        // Weights for the maximum that is known; where the tile has a score past it by more than 2^8, O and the
         // sum are rescaled and the weights, whose scores are still in registers, formed again.
         constexpr int Q = C::KT / 32;
         uint32_t v[Q][32];
-        tmem_ld32(ts, v[0]);
-        if (NP > 1) {  // the parts of P lie where scores are
 #pragma unroll
-            for (int j = 1; j < Q; ++j) tmem_ld32(ts + 32 * j, v[j]);
-        }
+        for (int j = 0; j < Q; ++j) tmem_ld32(ts + 32 * j, v[j]);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) tmem_wait_ld32(v[j]);  // one wait, and no barrier to the order of what follows
         float2 base = make_float2(PP_LIFT - m, PP_LIFT - m), sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         const float2 cc = make_float2(c, c);
         auto form = [&](int j) {
@@ -513,8 +512,6 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
         auto stream = [&](auto whole) {
 #pragma unroll
             for (int j = 0; j < Q; ++j) {
-                tmem_wait_ld32(v[j]);
-                if (NP == 1 && j + 1 < Q) tmem_ld32(ts + 32 * (j + 1), v[j + 1 < Q ? j + 1 : j]);
                 if (!decltype(whole)::value) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[j][e] = see[j] >> e & 1 ? v[j][e] : 0xff800000u;
