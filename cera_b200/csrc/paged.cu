@@ -123,6 +123,16 @@ int32_t paged_maps(const PagedView &kv, int type, uint32_t least, uint32_t *box,
     return tensor_map_4d(v, t, kv.v, dims, vs, boxes);
 }
 
+size_t paged_prefill_workspace(const PagedView &kv, int type, size_t n_heads, size_t n_tokens) {
+    return type == CERA_TYPE_F32 ? paged_prefill_f32_workspace(kv, n_heads, n_tokens) : paged_prefill_tc_workspace(kv, n_heads, n_tokens);
+}
+
+int32_t launch_paged_prefill(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
+                             PagedMask mask, void *out, void *ws, cudaStream_t st) {
+    if (type != CERA_TYPE_F32) return launch_paged_prefill_tc(kv, type, q, q_type, n_heads, starts, n_tokens, scale, mask, out, ws, st);
+    return launch_paged_prefill_f32(kv, (const float *)q, n_heads, starts, n_tokens, scale, mask, (float *)out, ws, st);
+}
+
 int32_t launch_paged_append(const PagedView &kv, int type, const void *k, const void *v, int src_type, const int32_t *starts, size_t n, float *weights,
                             int32_t *positions, size_t track_stride, const int32_t *token_pos, cudaStream_t st) {
     auto go = [&](auto cache, auto source) {

@@ -29,7 +29,11 @@ size_t paged_decode_workspace(const PagedView &kv, size_t n_heads, bool weights)
 int32_t launch_paged_decode(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, float scale, PagedMask mask, float *weights,
                             size_t weights_stride, void *out, void *ws, cudaStream_t st);
 size_t paged_prefill_workspace(const PagedView &kv, int type, size_t n_heads, size_t n_tokens);
-size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);  // 16-bit caches
+// 16-bit caches on the tensor cores, f32 caches with FMAs.
+size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);
+size_t paged_prefill_f32_workspace(const PagedView &kv, size_t n_heads, size_t n_tokens);
+int32_t launch_paged_prefill_f32(const PagedView &kv, const float *q, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale, PagedMask mask, float *out,
+                                 void *ws, cudaStream_t st);
 int32_t launch_paged_prefill_tc(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
                                 PagedMask mask, void *out, void *ws, cudaStream_t st);
 int32_t launch_paged_prefill(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,

@@ -15,10 +15,8 @@
 //
 // A row that ends without finite values - a weight of zero times an infinite value of a key it does not see, an infinity cut into parts - or
 // that has met no weight is computed again by paged_attend_row, which reads nothing that the row does not see.  Every wait is bounded.
-#include <algorithm>
-
 #include "mma.cuh"
-#include "paged.cuh"
+#include "paged_prefill.cuh"
 #include "tc.cuh"
 
 namespace cera {
@@ -34,20 +32,8 @@ static const bool g_paged_prefill_registered = register_kernel_status([] {
 namespace {
 
 constexpr uint32_t PP_ROWS = 128;
-constexpr float PP_FLOOR = -3.0e38f, PP_LIFT = 7.0f, PP_RAISE = 8.0f;
+constexpr float PP_LIFT = 7.0f, PP_RAISE = 8.0f;
 constexpr uint32_t PP_MASKS = 4;  // tiles whose masks are kept: more than the keys' stages and one
-
-struct PpParams {
-    PagedView kv;
-    PagedMask mask;
-    const void *q;
-    const int32_t *starts;
-    void *out;
-    float *part;   // [splits][tokens][heads][dim], for splits > 1
-    float2 *ml;    // [splits][tokens][heads]
-    float scale;
-    uint32_t n, heads, group, box;
-};
 
 // Shapes by the padded head size and the number of parts.
 template <int DP, int NP>
@@ -66,11 +52,6 @@ struct PpBars {
     uint64_t q_full, v_part, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], o_full[2];
 };
 
-__device__ __forceinline__ float pp_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float pp_max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -115,8 +96,6 @@ __device__ __forceinline__ uint64_t pp_desc_v(uint32_t addr, uint32_t block) {
 __device__ __forceinline__ uint32_t pp_idesc(bool bf, uint32_t N, bool n_major) {
     return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((n_major ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((PP_ROWS >> 4) << 24);
 }
-__device__ __forceinline__ uint32_t pp_low(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-
 template <typename T>
 __device__ __forceinline__ uint32_t pp_pack(float x, float y) {
     if (std::is_same<T, __half>::value) {
@@ -143,79 +122,6 @@ __device__ __forceinline__ void pp_parts(float x, float y, uint32_t (&w)[NP]) {
             y -= f.y;
         }
     }
-}
-
-// What a CTA works on: rows [row0, row0 + MT 128) of a (sequence, KV head), and of the key tiles that some of them sees [x0, x1).
-struct PpWork {
-    uint32_t s, row0, rows, t0, len;  // t0: the sequence's first token
-    int32_t p0;                       // the slot of its first token, negative if it has none
-    PagedSpan span;
-    uint32_t x0, x1;
-    int32_t lo0, lo1, hi0, hi1;  // of either tile of rows: the slots of its first and last row, and what the first's window begins with
-    uint32_t first0, first1;
-
-    __device__ __forceinline__ int32_t slot_of(uint32_t row, uint32_t group) const { return p0 + (int32_t)(row / group); }
-};
-
-// The unit-th run of MT tiles of all sequences, by a warp; false: there are not that many.
-template <int DP, int NP>
-__device__ __forceinline__ bool pp_find(const PpParams &p, PpWork &w, uint32_t unit) {
-    using C = Pp<DP, NP>;
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t ahead = 0;
-    for (uint32_t base = 0; base < p.kv.n_seqs; base += 32) {
-        const uint32_t s = base + lane;
-        uint32_t rows = 0;
-        if (s < p.kv.n_seqs) {
-            const int32_t a = min(max(p.starts[s], 0), (int32_t)p.n), b = min(max(p.starts[s + 1], a), (int32_t)p.n);
-            rows = (uint32_t)(b - a) * p.group;
-        }
-        const uint32_t units = (rows + C::MT * PP_ROWS - 1) / (C::MT * PP_ROWS);
-        uint32_t x = units;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= (uint32_t)o) x += y;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, ahead + x > unit);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            w.s = base + src;
-            w.rows = __shfl_sync(0xffffffffu, rows, src);
-            const uint32_t first = ahead + __shfl_sync(0xffffffffu, x - units, src), n = __shfl_sync(0xffffffffu, units, src);
-            w.row0 = (n - 1 - (unit - first)) * C::MT * PP_ROWS;  // the last rows see the most: first
-            return true;
-        }
-        ahead += __shfl_sync(0xffffffffu, x, 31);
-    }
-    return false;
-}
-
-template <int DP, int NP>
-__device__ __forceinline__ void pp_set(const PpParams &p, PpWork &w) {
-    using C = Pp<DP, NP>;
-    w.t0 = (uint32_t)min(max(p.starts[w.s], 0), (int32_t)p.n);
-    w.len = paged_len(p.kv, w.s);
-    w.p0 = (int32_t)w.len - (int32_t)(w.rows / p.group);
-    const uint32_t last = min(w.row0 + C::MT * PP_ROWS, w.rows) - 1;
-    w.span.set(p.mask, (uint32_t)max(w.slot_of(w.row0, p.group), 0), (uint32_t)max(w.slot_of(last, p.group) + 1, 0), C::KT);
-    auto tile = [&](uint32_t t, int32_t &lo, int32_t &hi, uint32_t &first) {
-        const uint32_t a = w.row0 + t * PP_ROWS;
-        const bool some = t < C::MT && a < w.rows;
-        lo = some ? w.slot_of(a, p.group) : -1;
-        hi = some ? w.slot_of(min(a + PP_ROWS, w.rows) - 1, p.group) : -1;
-        first = paged_first(p.mask, (uint32_t)max(lo, 0));
-    };
-    tile(0, w.lo0, w.hi0, w.first0);
-    tile(1, w.lo1, w.hi1, w.first1);
-    w.x0 = (uint32_t)((uint64_t)w.span.tiles * blockIdx.z / gridDim.z);
-    w.x1 = (uint32_t)((uint64_t)w.span.tiles * (blockIdx.z + 1) / gridDim.z);
-}
-
-// Whether tile t of the CTA's rows sees something of the key tile at slot0.
-template <int KT>
-__device__ __forceinline__ bool pp_sees(const PpParams &p, const PpWork &w, uint32_t t, uint32_t slot0) {
-    return (t ? w.hi1 : w.hi0) >= (int32_t)slot0 && (slot0 + KT > (t ? w.first1 : w.first0) || slot0 < p.mask.sink);
 }
 
 // The keys' or the values' loader, a warp.
@@ -615,8 +521,8 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     pdl_wait();
     if (warp == 0) {
         PpWork w;
-        const bool found = pp_find<DP, NP>(p, w, blockIdx.x);
-        if (found) pp_set<DP, NP>(p, w);
+        const bool found = pp_find<C::MT * PP_ROWS>(p, w, blockIdx.x);
+        if (found) pp_set<C::MT * PP_ROWS, PP_ROWS, C::KT>(p, w);
         else w.rows = 0;
         if (threadIdx.x == 0) {
             work = w;
@@ -669,63 +575,13 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     if (warp == C::MATH) tmem_dealloc(tmem, 512);
 }
 
-// A warp per row: the parts of its splits added up in their order.
-template <typename T, typename TQ>
-__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams p, uint32_t splits) {
-    pdl_trigger();
-    pdl_wait();
-    const uint32_t lane = threadIdx.x & 31;
-    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = (size_t)p.n * p.heads;
-    if (r >= all) return;
-    const uint32_t t = (uint32_t)(r / p.heads), h = (uint32_t)(r % p.heads), s = paged_seq_of(p.starts, p.kv.n_seqs, t);
-    if (s >= p.kv.n_seqs) return;
-    TQ *out = reinterpret_cast<TQ *>(p.out) + r * p.kv.dim;
-    const uint32_t len = paged_len(p.kv, s), behind = (uint32_t)p.starts[s + 1] - t;
-    if (behind > len) {
-        for (uint32_t d = lane; d < p.kv.dim; d += 32) out[d] = from_f32<TQ>(0.0f);
-        return;
-    }
-    float m = -INFINITY, l = 0.0f, o[8] = {};
-    for (uint32_t z = lane; z < splits; z += 32) m = fmaxf(m, p.ml[z * all + r].x);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-#pragma unroll 4
-    for (uint32_t z = 0; z < splits; ++z) {
-        const float2 v = p.ml[z * all + r];
-        if (v.x == -INFINITY) continue;
-        const float f = pp_exp2(v.x - m), *part = p.part + (z * all + r) * p.kv.dim;
-        l = fmaf(v.y, f, l);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (32 * i < p.kv.dim) o[i] = fmaf(part[lane + 32 * i], f, o[i]);
-    }
-    float check = l > 0.0f ? 0.0f : NAN;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (32 * i < p.kv.dim) {
-            check = fmaf(o[i] / l, 0.0f, check);
-            out[lane + 32 * i] = from_f32<TQ>(o[i] / l);
-        }
-    if (__any_sync(0xffffffffu, check != 0.0f))
-        paged_attend_row<T, TQ>(p.kv, p.mask, s, h / p.group, len - behind, reinterpret_cast<const TQ *>(p.q) + r * p.kv.dim, p.scale, out);
-}
-
-// CTAs along the rows (an upper bound: the portions' lengths are on the device) and the splits of the keys: as many as fill the SMs, of
-// four tiles of keys at least.
-struct PpGrid {
-    uint32_t units, splits;
-};
-PpGrid pp_grid(const PagedView &kv, size_t n_heads, size_t n) {
-    const size_t group = n_heads / kv.hk, rows = (kv.dim <= 128 ? 2 : 1) * PP_ROWS, units = std::min<size_t>(n * group / rows + std::min<size_t>(kv.n_seqs, n), n * group);
-    const size_t ctas = units * kv.hk, fit = (size_t)sm_count() / std::max<size_t>(ctas, 1), deep = (size_t)kv.max_pages * kv.page_size / 512;
-    return {(uint32_t)units, (uint32_t)std::max<size_t>(1, std::min(fit, deep))};
-}
+PpGrid pp_tc_grid(const PagedView &kv, size_t n_heads, size_t n) { return pp_grid(kv, n_heads, n, (kv.dim <= 128 ? 2 : 1) * PP_ROWS); }
 
 template <typename T, typename TQ, int DP>
 int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
     constexpr int NP = sizeof(TQ) == 2 ? 1 : std::is_same<T, __half>::value ? 2 : 3;
     using C = Pp<DP, NP>;
-    const PpGrid g = pp_grid(p.kv, p.heads, p.n);
+    const PpGrid g = pp_tc_grid(p.kv, p.heads, p.n);
     CUtensorMap mk, mv;
     p.box = C::KT;
     CERA_TRY(paged_maps(p.kv, type, 8, &p.box, &mk, &mv));
@@ -733,33 +589,18 @@ int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
     if (!by_tma) p.box = C::KT;
     auto kernel = by_tma ? paged_prefill_tc_kernel<T, TQ, DP, NP, true> : paged_prefill_tc_kernel<T, TQ, DP, NP, false>;
     CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
-    count_launch(g.splits > 1 ? 2 : 1);
+    count_launch();
     CERA_CUDA_TRY(launch_k(kernel, dim3(g.units, p.kv.hk, g.splits), dim3(C::THREADS), C::SMEM, st, mk, mv, p));
-    if (g.splits == 1) return CERA_CUDA_OK;
-    return check_cuda(launch_k(paged_prefill_join_kernel<T, TQ>, dim3((uint32_t)(((size_t)p.n * p.heads + 3) / 4)), dim3(128), 0, st, p, g.splits), "paged prefill join launch");
+    return pp_join<T, TQ>(p, g, st);
 }
 
 }  // namespace
 
-size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n) {
-    const PpGrid g = pp_grid(kv, n_heads, n);
-    return 16 + (g.splits > 1 ? g.splits * n * n_heads * ((size_t)kv.dim * 4 + 8) : 0);
-}
+size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n) { return pp_workspace(pp_tc_grid(kv, n_heads, n), kv, n_heads, n); }
 
 int32_t launch_paged_prefill_tc(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
                                 PagedMask mask, void *out, void *ws, cudaStream_t st) {
-    PpParams p;
-    p.kv = kv;
-    p.mask = mask;
-    p.q = q;
-    p.starts = starts;
-    p.out = out;
-    p.scale = scale;
-    p.n = (uint32_t)n_tokens;
-    p.heads = (uint32_t)n_heads;
-    p.group = p.heads / kv.hk;
-    p.part = (float *)ws;
-    p.ml = (float2 *)((uint8_t *)ws + (size_t)pp_grid(kv, n_heads, n_tokens).splits * n_tokens * n_heads * kv.dim * 4);
+    PpParams p = pp_params(kv, mask, q, n_heads, starts, n_tokens, scale, out, ws, pp_tc_grid(kv, n_heads, n_tokens));
     auto go = [&](auto cache, auto query) {
         using T = decltype(cache);
         using TQ = decltype(query);
