@@ -23,6 +23,18 @@ struct PagedMask {
 // until a page holds whole boxes.  0 where that would take it below `least`, or the pages are none or too far apart: no maps, rows are copied one by one.
 int32_t paged_maps(const PagedView &kv, int type, uint32_t least, uint32_t *box, CUtensorMap *k, CUtensorMap *v);
 
+// Lets a kernel have that much dynamic shared memory, asked for once per thread and device.
+template <auto KERNEL>
+inline int32_t paged_smem(size_t bytes) {
+    static thread_local int configured = -1;
+    int dev = 0;
+    CERA_CUDA_TRY(cudaGetDevice(&dev));
+    if (configured == dev) return CERA_CUDA_OK;
+    CERA_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    configured = dev;
+    return CERA_CUDA_OK;
+}
+
 int32_t launch_paged_append(const PagedView &kv, int type, const void *k, const void *v, int src_type, const int32_t *starts, size_t n, float *weights,
                             int32_t *positions, size_t track_stride, const int32_t *token_pos, cudaStream_t st);
 size_t paged_decode_workspace(const PagedView &kv, size_t n_heads, bool weights);

@@ -852,7 +852,8 @@ int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, 
     const bool by_tma = p.box != 0;
     if (!by_tma) p.box = W::TILE;
     auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, R, true> : paged_decode_kernel<T, TQ, DP, ST, R, false>;
-    CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    constexpr size_t most = PdSmem<W, DP, ST, sizeof(T) == 4>::FIXED + 4097 * 4;
+    CERA_TRY((by_tma ? paged_smem<paged_decode_kernel<T, TQ, DP, ST, R, true>>(most) : paged_smem<paged_decode_kernel<T, TQ, DP, ST, R, false>>(most)));
     count_launch(weights ? 3 : 2);
     CERA_CUDA_TRY(launch_k(kernel, dim3(G), dim3(PD_THREADS), smem, st, mk, mv, p));
     CERA_CUDA_TRY(launch_k(paged_join_kernel<TQ, W::TILE>, dim3(p.kv.n_seqs * p.kv.hk * p.chunks, std::min<uint32_t>(p.group, PD_ROWS)), dim3(PD_MATH), 0, st, p, G));

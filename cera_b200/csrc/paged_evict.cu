@@ -74,12 +74,55 @@ __device__ __forceinline__ void each_slot(const float *w, const int32_t *pos, ui
     }
 }
 
+constexpr uint32_t MOVE_SLOTS = 16;
+// A warp's MOVE_SLOTS slots from j0 on, a lane each with where its slot's content comes from (negative: nowhere): copies the key's and the value's row of those
+// that come from another slot, four at a time whose lookups and rows do not wait for one another.
+__device__ __forceinline__ void move_slots(const PagedView &kv, uint32_t s, uint32_t h, uint32_t row_bytes, uint32_t j0, int32_t from) {
+    constexpr int U = 4;
+    const uint32_t lane = threadIdx.x & 31, mine = j0 + lane;
+    uint32_t moved = __ballot_sync(0xffffffffu, from >= 0 && (uint32_t)from != mine);
+    while (moved) {
+        // lanes 0 to 3 look up the sources, 4 to 7 where they go
+        uint32_t i = 32, rest = moved;
+        for (uint32_t u = 0; u < (lane & 3) && rest; ++u) rest &= rest - 1;
+        if (rest) i = __ffs(rest) - 1;
+        const int32_t src = __shfl_sync(0xffffffffu, from, i & 31);
+        uint32_t row = 0, page = NO_PAGE;
+        if (lane < 8 && i < 32) page = paged_at(kv, s, lane < 4 ? (uint32_t)src : j0 + i, row);
+        for (int u = 0; u < U && moved; ++u) moved &= moved - 1;
+        uint32_t live = __ballot_sync(0xffffffffu, page != NO_PAGE);
+        live &= live >> 4 & 15;
+        if (!live) continue;
+        const uint8_t *from_k[U], *from_v[U];
+        uint8_t *to_k[U], *to_v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t p0 = __shfl_sync(0xffffffffu, page, u), r0 = __shfl_sync(0xffffffffu, row, u), p1 = __shfl_sync(0xffffffffu, page, u + 4), r1 = __shfl_sync(0xffffffffu, row, u + 4);
+            from_k[u] = kv.k + p0 * kv.k_page + r0 * kv.k_slot + h * kv.k_head;
+            from_v[u] = kv.v + p0 * kv.v_page + r0 * kv.v_slot + h * kv.v_head;
+            to_k[u] = kv.k + p1 * kv.k_page + r1 * kv.k_slot + h * kv.k_head;
+            to_v[u] = kv.v + p1 * kv.v_page + r1 * kv.v_slot + h * kv.v_head;
+        }
+        for (uint32_t b = lane * 16; b < 2 * row_bytes; b += 512) {
+            const bool is_v = b >= row_bytes;
+            const uint32_t o = is_v ? b - row_bytes : b;
+            uint4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (live >> u & 1) x[u] = *reinterpret_cast<const uint4 *>((is_v ? from_v[u] : from_k[u]) + o);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (live >> u & 1) *reinterpret_cast<uint4 *>((is_v ? to_v[u] : to_k[u]) + o) = x[u];
+        }
+    }
+}
+
 // With SMEM a thread owns `per` < 64 slots in a row, of which a 64-bit word each says which are kept; per is odd, so that the threads of a warp meet different
 // banks.
-template <bool SMEM>
+template <bool SMEM, bool MOVE>
 __global__ void __launch_bounds__(PICK_THREADS) paged_pick_kernel(const PagedView kv, const float *weights, const int32_t *positions, size_t stride, uint32_t budget,
                                                                   uint32_t n_sink, uint32_t n_recent, float *weights_out, int32_t *positions_out, size_t out_stride,
-                                                                  int32_t *kept) {
+                                                                  int32_t *kept, uint32_t row_bytes, int32_t *lens_out) {
     extern __shared__ uint32_t keys[];
     __shared__ uint32_t hist[PICK_BINS];
     __shared__ uint2 warps[PICK_WARPS];
@@ -94,6 +137,7 @@ __global__ void __launch_bounds__(PICK_THREADS) paged_pick_kernel(const PagedVie
     float *wo = weights_out + at * out_stride;
     int32_t *po = positions_out + at * out_stride, *ko = kept + at * budget;
     const uint32_t len = paged_len(kv, s);
+    if (MOVE && blockIdx.x == s * kv.hk && tid == 0) lens_out[s] = (int32_t)min(len, budget);
     for (uint32_t j = tid; j < budget; j += PICK_THREADS) ko[j] = j < len ? (int32_t)j : -1;
     if (len <= budget) {
         for (uint32_t j = tid; j < len; j += PICK_THREADS) {
@@ -232,54 +276,19 @@ __global__ void __launch_bounds__(PICK_THREADS) paged_pick_kernel(const PagedVie
                 po[j + u * PICK_THREADS] = b[u];
             }
     }
+    if (MOVE)
+        for (uint32_t j = warp * MOVE_SLOTS; j < budget; j += PICK_WARPS * MOVE_SLOTS)
+            move_slots(kv, s, blockIdx.x - s * kv.hk, row_bytes, j, lane < MOVE_SLOTS && j + lane < budget ? ko[j + lane] : -1);
 }
 
-// A warp per MOVE_SLOTS slots below the budget, a lane each; where a slot's content comes from another, the warp copies the key's and the value's row, four slots
-// at a time whose lookups and rows do not wait for one another.
-constexpr uint32_t MOVE_SLOTS = 16;
+// A warp per MOVE_SLOTS slots below the budget.
 __global__ void __launch_bounds__(256) paged_move_kernel(const PagedView kv, uint32_t row_bytes, uint32_t budget, const int32_t *__restrict__ kept, int32_t *lens_out) {
-    constexpr int U = 4;
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, s = blockIdx.y / kv.hk, h = blockIdx.y - s * kv.hk;
+    const uint32_t s = blockIdx.y / kv.hk, h = blockIdx.y - s * kv.hk;
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) lens_out[s] = (int32_t)min(paged_len(kv, s), budget);
-    const uint32_t j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * MOVE_SLOTS, mine = j0 + lane;
-    const int32_t from = lane < MOVE_SLOTS && mine < budget ? kept[(size_t)blockIdx.y * budget + mine] : -1;
-    uint32_t moved = __ballot_sync(0xffffffffu, from >= 0 && (uint32_t)from != mine);
-    while (moved) {
-        // lanes 0 to 3 look up the sources, 4 to 7 where they go
-        uint32_t i = 32, rest = moved;
-        for (uint32_t u = 0; u < (lane & 3) && rest; ++u) rest &= rest - 1;
-        if (rest) i = __ffs(rest) - 1;
-        const int32_t src = __shfl_sync(0xffffffffu, from, i & 31);
-        uint32_t row = 0, page = NO_PAGE;
-        if (lane < 8 && i < 32) page = paged_at(kv, s, lane < 4 ? (uint32_t)src : j0 + i, row);
-        for (int u = 0; u < U && moved; ++u) moved &= moved - 1;
-        uint32_t live = __ballot_sync(0xffffffffu, page != NO_PAGE);
-        live &= live >> 4 & 15;
-        if (!live) continue;
-        const uint8_t *from_k[U], *from_v[U];
-        uint8_t *to_k[U], *to_v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t p0 = __shfl_sync(0xffffffffu, page, u), r0 = __shfl_sync(0xffffffffu, row, u), p1 = __shfl_sync(0xffffffffu, page, u + 4), r1 = __shfl_sync(0xffffffffu, row, u + 4);
-            from_k[u] = kv.k + p0 * kv.k_page + r0 * kv.k_slot + h * kv.k_head;
-            from_v[u] = kv.v + p0 * kv.v_page + r0 * kv.v_slot + h * kv.v_head;
-            to_k[u] = kv.k + p1 * kv.k_page + r1 * kv.k_slot + h * kv.k_head;
-            to_v[u] = kv.v + p1 * kv.v_page + r1 * kv.v_slot + h * kv.v_head;
-        }
-        for (uint32_t b = lane * 16; b < 2 * row_bytes; b += 512) {
-            const bool is_v = b >= row_bytes;
-            const uint32_t o = is_v ? b - row_bytes : b;
-            uint4 x[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (live >> u & 1) x[u] = *reinterpret_cast<const uint4 *>((is_v ? from_v[u] : from_k[u]) + o);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (live >> u & 1) *reinterpret_cast<uint4 *>((is_v ? to_v[u] : to_k[u]) + o) = x[u];
-        }
-    }
+    const uint32_t lane = threadIdx.x & 31, j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * MOVE_SLOTS;
+    move_slots(kv, s, h, row_bytes, j0, lane < MOVE_SLOTS && j0 + lane < budget ? kept[(size_t)blockIdx.y * budget + j0 + lane] : -1);
 }
 
 }  // namespace
@@ -289,14 +298,20 @@ int32_t launch_paged_evict(const PagedView &kv, int type, const float *weights, 
                            cudaStream_t st) {
     const size_t cap = (size_t)kv.max_pages * kv.page_size, movers = cap > budget ? std::min(budget, cap - budget) : 0;
     const bool smem = cap + movers <= PICK_WORDS;
-    auto pick = smem ? paged_pick_kernel<true> : paged_pick_kernel<false>;
+    // few slots that can move: the CTA that picks them moves them, unless the lengths that all CTAs of a sequence read are overwritten (8 sequences of 2049 slots and 8
+    // heads: FUSED_A us with a second launch, FUSED_B without)
+    const bool move = smem && movers <= PICK_THREADS && (lens_out + kv.n_seqs <= kv.lens || kv.lens + kv.n_seqs <= lens_out);
+    auto pick = move ? paged_pick_kernel<true, true> : smem ? paged_pick_kernel<true, false> : paged_pick_kernel<false, false>;
     const size_t bytes = 4 * (smem ? cap + movers : 2 * (size_t)PICK_THREADS);
-    CERA_CUDA_TRY(cudaFuncSetAttribute(pick, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * PICK_WORDS)));
-    count_launch(2);
-    CERA_CUDA_TRY(launch_k(pick, dim3(kv.n_seqs * kv.hk), dim3(PICK_THREADS), bytes, st, kv, weights, positions, track_stride, (uint32_t)budget, n_sink, n_recent,
-                           weights_out, positions_out, out_stride, kept));
-    const uint32_t pairs = kv.n_seqs * kv.hk, wide = (uint32_t)((std::min(budget, cap) + 8 * MOVE_SLOTS - 1) / (8 * MOVE_SLOTS));
-    return check_cuda(launch_k(paged_move_kernel, dim3(std::max(1u, wide), pairs), dim3(256), 0, st, kv, kv.dim * (type == CERA_TYPE_F32 ? 4u : 2u), (uint32_t)budget, (const int32_t *)kept, lens_out),
+    if (smem) CERA_TRY((move ? paged_smem<paged_pick_kernel<true, true>>(4 * PICK_WORDS) : paged_smem<paged_pick_kernel<true, false>>(4 * PICK_WORDS)));
+    const uint32_t row_bytes = kv.dim * (type == CERA_TYPE_F32 ? 4u : 2u), pairs = kv.n_seqs * kv.hk;
+    count_launch();
+    CERA_CUDA_TRY(launch_k(pick, dim3(pairs), dim3(PICK_THREADS), bytes, st, kv, weights, positions, track_stride, (uint32_t)budget, n_sink, n_recent, weights_out,
+                           positions_out, out_stride, kept, row_bytes, lens_out));
+    if (move) return CERA_CUDA_OK;
+    const uint32_t wide = (uint32_t)((std::min(budget, cap) + 8 * MOVE_SLOTS - 1) / (8 * MOVE_SLOTS));
+    count_launch();
+    return check_cuda(launch_k(paged_move_kernel, dim3(std::max(1u, wide), pairs), dim3(256), 0, st, kv, row_bytes, (uint32_t)budget, (const int32_t *)kept, lens_out),
                       "paged evict launch");
 }
 

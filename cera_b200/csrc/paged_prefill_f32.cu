@@ -227,7 +227,7 @@ PpGrid pf_grid(const PagedView &kv, size_t n_heads, size_t n) { return pp_grid(k
 template <int DP>
 int32_t pf_launch(const PpParams &p, const PpGrid &g, cudaStream_t st) {
     auto kernel = paged_prefill_f32_kernel<DP>;
-    CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Pf<DP>::SMEM));
+    CERA_TRY(paged_smem<paged_prefill_f32_kernel<DP>>(Pf<DP>::SMEM));
     count_launch();
     CERA_CUDA_TRY(launch_k(kernel, dim3(g.units, p.kv.hk, g.splits), dim3(PF_THREADS), Pf<DP>::SMEM, st, p));
     return pp_join<float, float>(p, g, st);

@@ -588,7 +588,7 @@ int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
     const bool by_tma = p.box != 0;
     if (!by_tma) p.box = C::KT;
     auto kernel = by_tma ? paged_prefill_tc_kernel<T, TQ, DP, NP, true> : paged_prefill_tc_kernel<T, TQ, DP, NP, false>;
-    CERA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    CERA_TRY((by_tma ? paged_smem<paged_prefill_tc_kernel<T, TQ, DP, NP, true>>(C::SMEM) : paged_smem<paged_prefill_tc_kernel<T, TQ, DP, NP, false>>(C::SMEM)));
     count_launch();
     CERA_CUDA_TRY(launch_k(kernel, dim3(g.units, p.kv.hk, g.splits), dim3(C::THREADS), C::SMEM, st, mk, mv, p));
     return pp_join<T, TQ>(p, g, st);

@@ -14,18 +14,19 @@ from .types import BF16, F16, F32
 _TYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
-def _current():
-    return ops._device() if ops._device else torch.cuda.current_device()
-
-
-def _take(t, what, dtype, shape, device):
-    """t as a contiguous tensor of that type and shape (None: any extent) on the cache's device."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise TypeError(f"{what}: expected a tensor on {device}, where the cache is")
+def _refuse(t, what, dtype, shape, index):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
+        raise TypeError(f"{what}: expected a tensor on cuda:{index}, where the cache is")
     if t.dtype != dtype or not t.is_contiguous():
         raise TypeError(f"{what}: expected a contiguous {dtype} tensor, got {t.dtype}")
-    if t.dim() != len(shape) or any(a is not None and a != b for a, b in zip(shape, t.shape)):
-        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _take(t, what, dtype, shape, index):
+    """The address of t, which is a contiguous tensor of that type and shape on the cache's device.  (A small call takes about as long here as on the GPU: one
+    line of cheap questions, and the refusal's words apart.)"""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()):
+        _refuse(t, what, dtype, shape, index)
     return t.data_ptr()
 
 
@@ -58,7 +59,7 @@ class PagedKv:
         n_pages, page_size, n_kv_heads, head_dim = k_pages.shape
         self.n_seqs, self.n_kv_heads, self.head_dim, self.page_size = seq_lens.shape[0], n_kv_heads, head_dim, page_size
         self.capacity = page_table.shape[1] * page_size  # slots of a sequence
-        self.dtype, self.device = k_pages.dtype, k_pages.device
+        self.dtype, self.device, self.index = k_pages.dtype, k_pages.device, k_pages.get_device()
         # the stride of an extent of one is no stride
         ks, vs = ([st if n > 1 else 0 for n, st in zip(t.shape, t.stride())] for t in (k_pages, v_pages))
         self._desc = PagedKvDesc(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
@@ -66,22 +67,34 @@ class PagedKv:
         self._ref = C.byref(self._desc)
         self._workspace = {}
 
-    def _here(self):
-        if self.device.index != _current():
-            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{_current()}: make the cache's device current")
-        return self._ref
+    def _stream(self):
+        """The current stream, which is one of the cache's device."""
+        if ops._raw_stream and ops._device:
+            if ops._device() == self.index:
+                return ops._raw_stream(self.index)
+        elif torch.cuda.current_device() == self.index:
+            return torch.cuda.current_stream().cuda_stream
+        raise ValueError(f"the cache is on {self.device}, the current device is another: make the cache's current")
 
-    def _rows(self, t, what, shape):
-        """Rows of the cache's type or float32."""
-        if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
-            return _take(t, what, torch.float32, shape, self.device)
-        return _take(t, what, self.dtype, shape, self.device)
+    def _rows(self, t, what, n, heads):
+        """Rows [n][heads][head_dim] of the cache's type or float32 (None: as many as there are)."""
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            raise TypeError(f"{what}: expected a tensor of three dimensions")
+        shape = (t.shape[0] if n is None else n, t.shape[1] if heads is None else heads, self.head_dim)
+        return _take(t, what, torch.float32 if t.dtype is torch.float32 else self.dtype, shape, self.index)
 
-    def _track(self, t, what, dtype):
-        p = _take(t, what, dtype, (self.n_seqs, self.n_kv_heads, None), self.device)
-        if t.shape[2] < self.capacity:
-            raise ValueError(f"{what}: {t.shape[2]} slots, a sequence has {self.capacity}")
-        return p
+    def _track(self, t, what, dtype, least):
+        """Weights or positions [n_seqs][n_kv_heads][at least `least`] -> address and slots."""
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            raise TypeError(f"{what}: expected a tensor of three dimensions")
+        slots = t.shape[2]
+        p = _take(t, what, dtype, (self.n_seqs, self.n_kv_heads, slots), self.index)
+        if slots < least:
+            raise ValueError(f"{what}: {slots} slots, {least} needed")
+        return p, slots
+
+    def _starts(self, starts):
+        return _take(starts, "starts", torch.int32, (self.n_seqs + 1,), self.index)
 
     def _scratch(self, workspace, key, ask):
         need = self._workspace.get(key)
@@ -94,7 +107,7 @@ class PagedKv:
             self._workspace[key] = need
         if workspace is None:
             return torch.empty(need, dtype=torch.uint8, device=self.device)
-        _take(workspace, "workspace", torch.uint8, (None,), self.device)
+        _take(workspace, "workspace", torch.uint8, (workspace.numel(),) if isinstance(workspace, torch.Tensor) else (), self.index)
         if workspace.shape[0] < need:
             raise ValueError(f"workspace: {workspace.shape[0]} bytes, {need} needed")
         return workspace
@@ -105,32 +118,27 @@ def _visible(window, n_sink):
         raise ValueError(f"window {window} and n_sink {n_sink}: counts of slots")
 
 
-def _starts(cache, starts):
-    return None if starts is None else _take(starts, "starts", torch.int32, (cache.n_seqs + 1,), cache.device)
-
-
 def paged_append(cache, k, v, starts=None, weights=None, positions=None, token_positions=None):
     """Stores new tokens' keys and values, [n_tokens, n_kv_heads, head_dim] of the cache's type or float32 (rounded), in slots that
     seq_lens already counts: sequence s's tokens [starts[s], starts[s + 1]) - int32 [n_seqs + 1]; None: one token each - go to its last slots.
     Per slot and head, [n_seqs, n_kv_heads, at least capacity]: weights (float32) becomes 0, positions (int32) the token's position out of
     token_positions, int32 [n_tokens] (None: its slot)."""
-    ref = cache._here()
-    shape = (None, cache.n_kv_heads, cache.head_dim)
-    kp, vp = cache._rows(k, "k", shape), cache._rows(v, "v", shape)
+    stream = cache._stream()
+    kp = cache._rows(k, "k", None, cache.n_kv_heads)
     n = k.shape[0]
-    if v.shape[0] != n or v.dtype != k.dtype:
-        raise ValueError(f"k and v differ: {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    vp = _take(v, "v", k.dtype, (n, cache.n_kv_heads, cache.head_dim), cache.index)
     wp = pp = tp = None
     stride = 0
     if weights is not None:
-        wp, stride = cache._track(weights, "weights", torch.float32), weights.shape[2]
+        wp, stride = cache._track(weights, "weights", torch.float32, cache.capacity)
     if positions is not None:
-        pp, stride = cache._track(positions, "positions", torch.int32), positions.shape[2]
-        if weights is not None and weights.shape[2] != stride:
+        pp, slots = cache._track(positions, "positions", torch.int32, cache.capacity)
+        if weights is not None and slots != stride:
             raise ValueError("weights and positions differ in their slots")
+        stride = slots
     if token_positions is not None:
-        tp = _take(token_positions, "token_positions", torch.int32, (n,), cache.device)
-    check(lib.cera_cuda_paged_append(ref, kp, vp, _TYPE[k.dtype], _starts(cache, starts), n, wp, pp, stride, tp, ops._stream()))
+        tp = _take(token_positions, "token_positions", torch.int32, (n,), cache.index)
+    check(lib.cera_cuda_paged_append(cache._ref, kp, vp, _TYPE[k.dtype], None if starts is None else cache._starts(starts), n, wp, pp, stride, tp, stream))
 
 
 def paged_decode_attention(cache, q, scale, window=0, n_sink=0, weights=None, out=None, workspace=None):
@@ -138,20 +146,18 @@ def paged_decode_attention(cache, q, scale, window=0, n_sink=0, weights=None, ou
     the result is of q's type.  window: only that many last slots are seen, and the first n_sink (0: all).  weights, float32
     [n_seqs, n_kv_heads, at least capacity], has the probabilities of a KV head's query heads added to their slots.  A sequence
     without slots gives zeros.  Calls that may overlap need a workspace each; by default every call has its own."""
-    ref = cache._here()
-    qp = cache._rows(q, "q", (cache.n_seqs, None, cache.head_dim))
+    stream, ref = cache._stream(), cache._ref
+    qp = cache._rows(q, "q", cache.n_seqs, None)
     _visible(window, n_sink)
     heads, stride, wp = q.shape[1], 0, None
     if weights is not None:
-        wp, stride = cache._track(weights, "weights", torch.float32), weights.shape[2]
+        wp, stride = cache._track(weights, "weights", torch.float32, cache.capacity)
     if out is None:
         out = torch.empty_like(q)
     else:
-        _take(out, "out", q.dtype, q.shape, cache.device)
-    ws = cache._scratch(workspace, ("decode", heads, wp is not None),
-                        lambda: lib.cera_cuda_paged_decode_attention_workspace_bytes(ref, heads, int(wp is not None)))
-    check(lib.cera_cuda_paged_decode_attention(ref, qp, _TYPE[q.dtype], heads, scale, window, n_sink, wp, stride, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                               ops._stream()))
+        _take(out, "out", q.dtype, q.shape, cache.index)
+    ws = cache._scratch(workspace, (heads, wp is not None), lambda: lib.cera_cuda_paged_decode_attention_workspace_bytes(ref, heads, int(wp is not None)))
+    check(lib.cera_cuda_paged_decode_attention(ref, qp, _TYPE[q.dtype], heads, scale, window, n_sink, wp, stride, out.data_ptr(), ws.data_ptr(), ws.shape[0], stream))
     return out
 
 
@@ -159,20 +165,16 @@ def paged_prefill_attention(cache, q, starts, scale, window=0, n_sink=0, out=Non
     """Causal attention of portions of prompts: q [n_tokens, n_heads, head_dim], of which sequence s has [starts[s], starts[s + 1])
     (int32 [n_seqs + 1], ascending from 0) in its last slots.  Types, window and n_sink as in paged_decode_attention, the window counted
     back from each query.  Rows past starts[n_seqs] are left as they are in `out`, and undefined without one."""
-    ref = cache._here()
-    qp = cache._rows(q, "q", (None, None, cache.head_dim))
-    if starts is None:
-        raise TypeError("starts: expected an int32 tensor")
+    stream, ref = cache._stream(), cache._ref
+    qp, sp = cache._rows(q, "q", None, None), cache._starts(starts)
     _visible(window, n_sink)
-    sp = _starts(cache, starts)
     n, heads = q.shape[0], q.shape[1]
     if out is None:
         out = torch.empty_like(q)
     else:
-        _take(out, "out", q.dtype, q.shape, cache.device)
-    ws = cache._scratch(workspace, ("prefill", heads, n), lambda: lib.cera_cuda_paged_prefill_attention_workspace_bytes(ref, heads, n))
-    check(lib.cera_cuda_paged_prefill_attention(ref, qp, _TYPE[q.dtype], heads, sp, n, scale, window, n_sink, out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                ops._stream()))
+        _take(out, "out", q.dtype, q.shape, cache.index)
+    ws = cache._scratch(workspace, (n, heads, None), lambda: lib.cera_cuda_paged_prefill_attention_workspace_bytes(ref, heads, n))
+    check(lib.cera_cuda_paged_prefill_attention(ref, qp, _TYPE[q.dtype], heads, sp, n, scale, window, n_sink, out.data_ptr(), ws.data_ptr(), ws.shape[0], stream))
     return out
 
 
@@ -184,21 +186,21 @@ def paged_evict(cache, weights, positions, budget, n_sink=0, n_recent=0, weights
     weights_out and positions_out (at least min(budget, capacity) slots).  kept, int32 [n_seqs, n_kv_heads, budget]: the slot that each slot's
     content came from, -1 past the length; seq_lens: min(length, budget) in a new tensor or in seq_lens_out, which may be
     cache.seq_lens.  Pages past the budget are the caller's again."""
-    ref = cache._here()
-    wp, pp = cache._track(weights, "weights", torch.float32), cache._track(positions, "positions", torch.int32)
-    shape = (cache.n_seqs, cache.n_kv_heads, None)
-    weights_out, positions_out = weights if weights_out is None else weights_out, positions if positions_out is None else positions_out
-    wo, po = _take(weights_out, "weights_out", torch.float32, shape, cache.device), _take(positions_out, "positions_out", torch.int32, shape, cache.device)
-    if weights.shape != positions.shape or weights_out.shape != positions_out.shape:
-        raise ValueError("weights and positions differ in their slots")
+    stream = cache._stream()
     _visible(n_recent, n_sink)
     if not n_sink + n_recent <= budget < 2**31 - 256 or budget < 1:
         raise ValueError(f"a budget of {budget} slots for {n_sink} first and {n_recent} recent ones")
+    wp, slots = cache._track(weights, "weights", torch.float32, cache.capacity)
+    pp, also = cache._track(positions, "positions", torch.int32, cache.capacity)
+    least = min(budget, cache.capacity)
+    wo, slots_out = (wp, slots) if weights_out is None else cache._track(weights_out, "weights_out", torch.float32, least)
+    po, also_out = (pp, also) if positions_out is None else cache._track(positions_out, "positions_out", torch.int32, least)
+    if slots != also or slots_out != also_out:
+        raise ValueError("weights and positions differ in their slots")
     kept = torch.empty((cache.n_seqs, cache.n_kv_heads, budget), dtype=torch.int32, device=cache.device)
     if seq_lens_out is None:
         seq_lens_out = torch.empty_like(cache.seq_lens)
     else:
-        _take(seq_lens_out, "seq_lens_out", torch.int32, (cache.n_seqs,), cache.device)
-    check(lib.cera_cuda_paged_evict(ref, wp, pp, weights.shape[2], budget, n_sink, n_recent, wo, po, weights_out.shape[2], kept.data_ptr(),
-                                    seq_lens_out.data_ptr(), ops._stream()))
+        _take(seq_lens_out, "seq_lens_out", torch.int32, (cache.n_seqs,), cache.index)
+    check(lib.cera_cuda_paged_evict(cache._ref, wp, pp, slots, budget, n_sink, n_recent, wo, po, slots_out, kept.data_ptr(), seq_lens_out.data_ptr(), stream))
     return kept, seq_lens_out
