@@ -63,15 +63,15 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pairs(void (*kernel)(KArgs...), uint32_t pairs, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), uint32_t ctas, uint32_t clusters, dim3 block, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * pairs);
+    cfg.gridDim = dim3(ctas * clusters);
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -79,6 +79,10 @@ inline cudaError_t launch_pairs(void (*kernel)(KArgs...), uint32_t pairs, dim3 b
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pairs(void (*kernel)(KArgs...), uint32_t pairs, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+    return launch_clusters(kernel, 2, pairs, block, smem, st, args...);
 }
 
 // ---- two CTAs of a cluster on one tile (cta_group::2).  Both allocate; the even CTA's thread issues the products, which read both CTAs'

@@ -322,9 +322,9 @@ def test_evict(dtype, in_place, ties, special, mixed):
 
 
 @pytest.mark.parametrize("in_place", [False, True])
-@pytest.mark.parametrize("length,budget", [(1025, 1024), (5000, 700), (31000, 4000), (70000, 66000), (70001, 500)])
+@pytest.mark.parametrize("length,budget", [(1025, 1024), (5000, 700), (31000, 4000), (70000, 66000), (70001, 500), (230001, 200000), (430001, 100000)])
 def test_evict_long(length, budget, in_place):
-    """Up to lengths whose keys do not fit in shared memory."""
+    """One CTA, clusters, and lengths whose keys do not fit in their shared memory."""
     need_gpu()
     import cera_b200 as cb
     c = R.Cache([0], 1, 32, 64, F16)
