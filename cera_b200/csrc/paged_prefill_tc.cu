@@ -9,7 +9,10 @@
 // is too: the warpgroup that finds a maximum raised by more than 2^8 rescales O on the spot.
 //
 // f32 queries over a 16-bit cache: the query and the weights enter as sums of NP parts of the cache's type (two f16, 22 bits; three
-// bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.
+// bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.  The tensor cores cut a sum at every step instead of rounding it, which
+// a long row would show (5500 slots in one sum: 4.7e-6 off for f16 and 6.6e-6 for bf16, 1.5e-6 with torch's f32 products): the least parts of the queries come first, and after
+// 128 slots O is added to an f32 sum and begun anew (8.7e-7 and 8.9e-7; 1500 queries of 32 heads over them 329 -> 353 us and 587 -> 576).  That sum is in TMEM as far as there is room:
+// all of it in local memory takes 536 and 709 us, whose bytes all come from L2.
 //
 // Few rows over a long cache: the keys are split over gridDim.z CTAs and paged_prefill_join_kernel adds the parts up.
 //
@@ -43,6 +46,8 @@ struct Pp {
     static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
     static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
     static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((NP * P_COLS > KT ? NP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
+    static constexpr uint32_t FLUSH = 128 / KT;  // tiles that O adds up with f32 queries
+    static constexpr uint32_t SPARE = (512 - MT * T_COLS) / MT / 32 * 32, KEPT = NP == 1 ? 0 : SPARE < DP ? SPARE : DP;  // numbers of a row's sum that TMEM has room for
     static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 4);  // warpgroups: softmax of a tile each; products, two loaders and a warp of nothing
     static constexpr size_t SMEM = 1024 + (size_t)MT * NP * QPART + (size_t)ST * 2 * HALF;
     static_assert(ST >= 1 && MT * T_COLS <= 512, "does not fit");
@@ -244,7 +249,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
         const uint64_t kd = k0 + st * (C::HALF / 16);
 #pragma unroll 1
         for (int part = 0; part < NP; ++part) {
-            const uint64_t qd = q0 + (t * NP + part) * (C::QPART / 16);
+            const uint64_t qd = q0 + (t * NP + NP - 1 - part) * (C::QPART / 16);  // the least first: sums are cut, not rounded, at every step
 #pragma unroll
             for (uint32_t k = 0; k < DP / 16; ++k)
                 if (k < steps) tc_mma_f16(d, qd + (k >> 2) * (C::QBLOCK / 16) + 2 * (k & 3), kd + (k >> 2) * (C::KBLOCK / 16) + 2 * (k & 3), id_s, part | k, me);
@@ -283,7 +288,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
 #pragma unroll 1
                 for (int part = 0; part < NP; ++part)
 #pragma unroll
-                    for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] | part | k, me);
+                    for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, (NP == 1 ? added[t] : added[t] % C::FLUSH) | part | k, me);
                 ++added[t];
             }
             if (t + 1 == C::MT) tc_commit(&b->v_empty[st], me);
@@ -368,12 +373,55 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     float m = PP_FLOOR, l = 0.0f;
     uint32_t done = 0;
     bool ok = true;
+    // with f32 queries: the sums of whole groups of FLUSH tiles, the first KEPT numbers in TMEM and the others in local memory
+    const uint32_t ta = tmem + C::MT * C::T_COLS + t * C::KEPT + (quad * 32 << 16);
+    constexpr int FAR = NP == 1 ? 0 : DP - (int)C::KEPT;
+    alignas(16) float far[FAR ? FAR : 1];
+    // f(number, its sum) for every number of the row, 32 at a time
+    auto sums = [&](auto f) {
+#pragma unroll
+        for (int d = 0; d < (int)C::KEPT; d += 32) {
+            if ((uint32_t)d >= p.kv.dim) break;
+            uint32_t s[32];
+            tmem_ld32(ta + d, s);
+            tmem_wait_ld32(s);
+            f(d, s);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t x[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = s[16 * h + e];
+                tmem_st16(ta + d + 16 * h, x);
+            }
+        }
+        if (C::KEPT) tmem_wait_st();
+#pragma unroll
+        for (int d = 0; d < FAR; d += 32) {
+            if (C::KEPT + d >= p.kv.dim) break;
+            uint32_t s[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(far[d + e]);
+            f(C::KEPT + d, s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) far[d + e] = __uint_as_float(s[e]);
+        }
+    };
+    auto flush = [&] {
+        sums([&](uint32_t d, uint32_t (&s)[32]) {
+            uint32_t o[32];
+            tmem_ld32(to + d, o);
+            tmem_wait_ld32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = done == C::FLUSH ? o[e] : __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(o[e]));
+        });
+    };
     for (uint32_t i = 0; i < w.x1 - w.x0; ++i) {
         const uint32_t slot0 = w.span.slot(w.x0 + i, C::KT);
         if (!pp_sees<C::KT>(p, w, t, slot0)) continue;
         ok = tma::mbar_wait_warp(&b->s_full[t], done & 1, abort_flag, status, 4u);
         if (!ok) break;
         tc_fence_after();
+        if (NP > 1 && done && done % C::FLUSH == 0) flush();  // O is complete up to the tile before, and begins anew
         // which of the tile's keys this row sees; nothing to look at where every row sees all
         uint32_t see[(C::KT + 31) / 32];
         bool all = (int32_t)(slot0 + C::KT) <= p_lo + 1 && ((int32_t)slot0 >= first_hi || slot0 + C::KT <= p.mask.sink);
@@ -437,6 +485,11 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             const float f = raise ? pp_exp2(m - mx) : 1.0f;
             if (raise) m = mx;
             l *= f;
+            if (NP > 1 && done >= C::FLUSH)
+                sums([&](uint32_t, uint32_t (&s)[32]) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
+                });
             for (uint32_t d = 0; done && d < p.kv.dim; d += 16) {  // O is complete up to the tile before, and nothing adds to it
                 uint32_t o[16];
                 tmem_ld16(to + d, o);
@@ -460,6 +513,20 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     if (ok && done) ok = tma::mbar_wait_warp(&b->o_full[t], 0, abort_flag, status, 4u);
     if (!ok) return;
     tc_fence_after();
+    if (NP > 1 && done > C::FLUSH) {  // O joins the sums
+        sums([&](uint32_t d, uint32_t (&s)[32]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t o[16];
+                tmem_ld16(to + d + 16 * h, o);
+                tmem_wait_ld16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(s[16 * h + e]) + __uint_as_float(o[e]));
+                tmem_st16(to + d + 16 * h, o);
+            }
+        });
+        tmem_wait_st();
+    }
     const size_t place = ((size_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group);
     if (gridDim.z > 1) {
         const size_t at = (size_t)blockIdx.z * p.n * p.heads + place;

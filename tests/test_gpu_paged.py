@@ -170,6 +170,36 @@ def test_prefill_several_tiles(types, dim):
     _prefill_case(cb, c, 3, types[0], [300], window=190, sink=5)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 224])
+@pytest.mark.parametrize("growing", [False, True])
+def test_prefill_f32_over_many_slots(dtype, dim, growing):
+    """Sums of many slots keep the precision of f32: with values of one sign, cutting a sum at each of its 2500 or 3750 steps by 2^-24 on average would add up to 1e-4.
+    Bound, relative to the result's norm: scores of size 4 in dim / 16 <= 14 steps of 2^-23, which enter twice (above and below the line), 1.4e-5; sums of 128 slots in
+    24 steps of 2^-23, 2.9e-6; 160 groups in steps of 2^-24 at random signs and parts of 2^-22, 1e-6.
+    `growing`: scores that rise along the slots to 64 (2e-4 by the first term), so that the maximum is raised after sums were put aside."""
+    need_gpu()
+    import cera_b200 as cb
+    n, heads, slots, page = 700, 16, 20000, 32
+    g = torch.Generator("cuda").manual_seed(dim)
+    k = torch.randn(slots // page, page, 2, dim, generator=g, device="cuda")
+    if growing:
+        k[..., 0] = torch.arange(slots, device="cuda").reshape(-1, page, 1) * (60.0 / slots)
+    k, v = k.to(dtype), (torch.rand(slots // page, page, 2, dim, generator=g, device="cuda") + 0.5).to(dtype)
+    q = torch.randn(n, heads, dim, generator=g, device="cuda")
+    if growing:
+        q[..., 0] = math.sqrt(dim)
+    table = torch.randperm(slots // page, generator=torch.Generator().manual_seed(1)).to(torch.int32)[None].cuda()
+    cache = cb.PagedKv(k, v, table, torch.tensor([slots], dtype=torch.int32, device="cuda"))
+    got = cb.paged_prefill_attention(cache, q, torch.tensor([0, n], dtype=torch.int32, device="cuda"), 1.0 / math.sqrt(dim))
+    kk, vv = (x[table[0].long()].reshape(slots, 2, dim).double() for x in (k, v))
+    hidden = torch.arange(slots, device="cuda") > torch.arange(slots - n, slots, device="cuda")[:, None]
+    for h in range(0, heads, 5):
+        x = (q[:, h].double() @ kk[:, h // 8].T / math.sqrt(dim)).masked_fill_(hidden, -math.inf)
+        want = torch.softmax(x, -1) @ vv[:, h // 8]
+        assert float((got[:, h].double() - want).norm() / want.norm()) < (2.2e-4 if growing else 2e-5)
+
+
 def test_prefill_of_more_tokens_than_are_cached():
     """Queries whose place is before the first slot see nothing."""
     need_gpu()
