@@ -71,7 +71,7 @@ __device__ __forceinline__ uint64_t pd_start(uint32_t b, uint64_t total, uint64_
 
 // The tiles of the call in one line, each unit's behind a stretch of PD_BEGIN that stands for what a unit costs beside its tiles (its queries, and
 // the warps' meeting at its end): without it a CTA that got many short units took twice as long as the rest (24 sequences of 1 to 9000 slots
-// TIME_A us, with it TIME_B).  Where every tile has a CTA of its own there is none.  sums live in shared memory.
+// 70 us, with it 39).  Where every tile has a CTA of its own there is none.  sums live in shared memory.
 struct PdLine {
     const uint32_t *sums;        // the line ahead of sequence s, of one unit each; sums[n] is all
     uint32_t n, per_seq, begin;  // units of a sequence; a unit's stretch

@@ -492,14 +492,14 @@ __global__ void __launch_bounds__(PICK_THREADS) paged_pick_far_kernel(const Page
     }
 }
 
-// A warp per MOVE_SLOTS slots below the budget.
+// A warp per MOVE_SLOTS slots below the budget, a row of CTAs per pair.
 __global__ void __launch_bounds__(256) paged_move_kernel(const PagedView kv, uint32_t row_bytes, uint32_t budget, const int32_t *__restrict__ kept, int32_t *lens_out) {
     pdl_trigger();
     pdl_wait();
-    const uint32_t s = blockIdx.y / kv.hk, h = blockIdx.y - s * kv.hk;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) lens_out[s] = (int32_t)min(paged_len(kv, s), budget);
-    const uint32_t lane = threadIdx.x & 31, j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * MOVE_SLOTS;
-    move_slots(kv, s, h, row_bytes, j0 + lane, lane < MOVE_SLOTS && j0 + lane < budget ? kept[(size_t)blockIdx.y * budget + j0 + lane] : -1);
+    const uint32_t s = blockIdx.x / kv.hk, h = blockIdx.x - s * kv.hk, lane = threadIdx.x & 31;
+    if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0) lens_out[s] = (int32_t)min(paged_len(kv, s), budget);
+    for (uint32_t j0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * MOVE_SLOTS; j0 < budget; j0 += gridDim.y * 8 * MOVE_SLOTS)
+        move_slots(kv, s, h, row_bytes, j0 + lane, lane < MOVE_SLOTS && j0 + lane < budget ? kept[(size_t)blockIdx.x * budget + j0 + lane] : -1);
 }
 
 }  // namespace
@@ -537,9 +537,10 @@ int32_t launch_paged_evict(const PagedView &kv, int type, const float *weights, 
                                positions_out, out_stride, kept));
     }
     if (move) return CERA_CUDA_OK;
-    const uint32_t wide = (uint32_t)((std::min(budget, cap) + 8 * MOVE_SLOTS - 1) / (8 * MOVE_SLOTS));
+    const size_t wide = (std::min(budget, cap) + 8 * MOVE_SLOTS - 1) / (8 * MOVE_SLOTS);
     count_launch();
-    return check_cuda(launch_k(paged_move_kernel, dim3(std::max(1u, wide), pairs), dim3(256), 0, st, kv, row_bytes, (uint32_t)budget, (const int32_t *)kept, lens_out),
+    return check_cuda(launch_k(paged_move_kernel, dim3(pairs, (uint32_t)std::min<size_t>(std::max<size_t>(1, wide), 65535)), dim3(256), 0, st, kv, row_bytes, (uint32_t)budget,
+                               (const int32_t *)kept, lens_out),
                       "paged evict launch");
 }
 
