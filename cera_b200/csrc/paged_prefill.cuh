@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 #include "paged.cuh"
 
@@ -144,19 +145,45 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams 
         paged_attend_row<T, TQ>(p.kv, p.mask, s, h / p.group, len - behind, reinterpret_cast<const TQ *>(p.q) + r * p.kv.dim, p.scale, out);
 }
 
-// CTAs along the rows (an upper bound: the portions' lengths are on the device) and the splits of the keys: as many as fill the SMs, of
-// four tiles of keys at least.
+// CTAs along the rows (an upper bound: the portions' lengths are on the device) and the splits of the keys.
 struct PpGrid {
     uint32_t units, splits;
 };
-inline PpGrid pp_grid(const PagedView &kv, size_t n_heads, size_t n, size_t rows) {
-    const size_t group = n_heads / kv.hk, units = std::min<size_t>(n * group / rows + std::min<size_t>(kv.n_seqs, n), n * group);
-    const size_t ctas = units * kv.hk, fit = (size_t)sm_count() / std::max<size_t>(ctas, 1), deep = (size_t)kv.max_pages * kv.page_size / 512;
-    return {(uint32_t)units, (uint32_t)std::max<size_t>(1, std::min(fit, deep))};
+// Microseconds that a run of rows takes with 64 slots, and beside all of them (its queries, its result, the launch).
+struct PpCost {
+    float slots, beside;
+};
+constexpr size_t PP_PARTS = (size_t)256 << 20;  // bytes of parts, at most
+
+// The splits with which the call should be done first, as far as the host knows the lengths: capacity slots a sequence, the new tokens its last ones.  Where they are few, CTAs
+// see alike and come in whole turns of the SMs (152 CTAs of 300 f32 tokens over 2000 slots: 659 us unsplit, 459 so); where they are most of the slots, a CTA sees half of
+// them on average and the longest counts.  Parts are written, and read by the join.
+inline uint32_t pp_splits(const PagedView &kv, size_t n_heads, size_t n, size_t rows, size_t units, PpCost cost, PagedMask mask) {
+    const size_t cap = std::max<size_t>(1, (size_t)kv.max_pages * kv.page_size), seqs = std::max<size_t>(1, std::min<size_t>(kv.n_seqs, n));
+    size_t longest = cap;
+    if (mask.window) longest = std::min<size_t>(cap, (size_t)mask.window + std::min<size_t>(mask.sink, cap) + rows * kv.hk / n_heads + 64);
+    const float tiles = (float)((longest + 63) / 64), turns = (float)(units * kv.hk) / sm_count(), spread = mask.window ? 0.0f : std::min(1.0f, (float)n / seqs / cap);
+    const float join = 0.15f + (float)n * n_heads * kv.dim * 8 / 4e6f;  // a part: a turn of the join's loop, and its bytes at 4 TB/s
+    const size_t most = std::min<size_t>({(size_t)tiles, 64, std::max<size_t>(1, PP_PARTS / (n * n_heads * ((size_t)kv.dim * 4 + 8)))});
+    float best = 0.0f;
+    uint32_t splits = 1;
+    for (uint32_t z = 1; z <= most; ++z) {
+        const float each = std::ceil(tiles / z) * cost.slots, alike = std::ceil(turns * z) * (each + cost.beside),
+                    mixed = std::max(each + cost.beside, turns * z * (each / 2 + cost.beside) + each / 2), t = alike + spread * (mixed - alike) + (z > 1 ? 3.0f + z * join : 0.0f);
+        if (z == 1 || t < 0.97f * best) {
+            best = t;
+            splits = z;
+        }
+    }
+    return splits;
+}
+inline size_t pp_units(const PagedView &kv, size_t n_heads, size_t n, size_t rows) {
+    const size_t group = n_heads / kv.hk;
+    return std::min<size_t>(n * group / rows + std::min<size_t>(kv.n_seqs, n), n * group);
 }
 
-inline size_t pp_workspace(const PpGrid &g, const PagedView &kv, size_t n_heads, size_t n) {
-    return 16 + (g.splits > 1 ? g.splits * n * n_heads * ((size_t)kv.dim * 4 + 8) : 0);
+inline size_t pp_workspace(uint32_t splits, const PagedView &kv, size_t n_heads, size_t n) {
+    return 16 + (splits > 1 ? splits * n * n_heads * ((size_t)kv.dim * 4 + 8) : 0);
 }
 
 inline PpParams pp_params(const PagedView &kv, PagedMask mask, const void *q, size_t n_heads, const int32_t *starts, size_t n, float scale, void *out, void *ws,

@@ -222,7 +222,9 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
     }
 }
 
-PpGrid pf_grid(const PagedView &kv, size_t n_heads, size_t n) { return pp_grid(kv, n_heads, n, PF_ROWS); }
+uint32_t pf_splits(const PagedView &kv, size_t n_heads, size_t n, PagedMask mask) {
+    return pp_splits(kv, n_heads, n, PF_ROWS, pp_units(kv, n_heads, n, PF_ROWS), PpCost{0.08f * kv.dim, 8.0f}, mask);
+}
 
 template <int DP>
 int32_t pf_launch(const PpParams &p, const PpGrid &g, cudaStream_t st) {
@@ -235,11 +237,13 @@ int32_t pf_launch(const PpParams &p, const PpGrid &g, cudaStream_t st) {
 
 }  // namespace
 
-size_t paged_prefill_f32_workspace(const PagedView &kv, size_t n_heads, size_t n) { return pp_workspace(pf_grid(kv, n_heads, n), kv, n_heads, n); }
+size_t paged_prefill_f32_workspace(const PagedView &kv, size_t n_heads, size_t n) { return pp_workspace(pf_splits(kv, n_heads, n, PagedMask{0, 0}), kv, n_heads, n); }
 
 int32_t launch_paged_prefill_f32(const PagedView &kv, const float *q, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale, PagedMask mask, float *out,
                                  void *ws, cudaStream_t st) {
-    const PpGrid g = pf_grid(kv, n_heads, n_tokens);
+    uint32_t splits = pf_splits(kv, n_heads, n_tokens, mask);
+    if (mask.window) splits = std::min(splits, pf_splits(kv, n_heads, n_tokens, PagedMask{0, 0}));  // which the workspace has room for
+    const PpGrid g = {(uint32_t)pp_units(kv, n_heads, n_tokens, PF_ROWS), splits};
     const PpParams p = pp_params(kv, mask, q, n_heads, starts, n_tokens, scale, out, ws, g);
     if (kv.dim <= 64) return pf_launch<64>(p, g, st);
     if (kv.dim <= 128) return pf_launch<128>(p, g, st);

@@ -642,13 +642,23 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     if (warp == C::MATH) tmem_dealloc(tmem, 512);
 }
 
-PpGrid pp_tc_grid(const PagedView &kv, size_t n_heads, size_t n) { return pp_grid(kv, n_heads, n, (kv.dim <= 128 ? 2 : 1) * PP_ROWS); }
+// np: parts of a query.
+uint32_t pp_tc_splits(const PagedView &kv, size_t n_heads, size_t n, int np, PagedMask mask) {
+    const size_t rows = (kv.dim <= 128 ? 2 : 1) * PP_ROWS;
+    const PpCost cost = {(np == 1 ? 1.05f : np == 2 ? 2.3f : 3.7f) * kv.dim / 128, np == 1 ? 9.0f : 14.0f};
+    return pp_splits(kv, n_heads, n, rows, pp_units(kv, n_heads, n, rows), cost, mask);
+}
+// With any queries and mask.
+uint32_t pp_tc_most(const PagedView &kv, size_t n_heads, size_t n) {
+    uint32_t most = 1;
+    for (int np = 1; np <= 3; ++np) most = std::max(most, pp_tc_splits(kv, n_heads, n, np, PagedMask{0, 0}));
+    return most;
+}
 
 template <typename T, typename TQ, int DP>
-int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
+int32_t pp_launch(PpParams &p, const PpGrid &g, int type, cudaStream_t st) {
     constexpr int NP = sizeof(TQ) == 2 ? 1 : std::is_same<T, __half>::value ? 2 : 3;
     using C = Pp<DP, NP>;
-    const PpGrid g = pp_tc_grid(p.kv, p.heads, p.n);
     CUtensorMap mk, mv;
     p.box = C::KT;
     CERA_TRY(paged_maps(p.kv, type, 8, &p.box, &mk, &mv));
@@ -663,17 +673,21 @@ int32_t pp_launch(PpParams &p, int type, cudaStream_t st) {
 
 }  // namespace
 
-size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n) { return pp_workspace(pp_tc_grid(kv, n_heads, n), kv, n_heads, n); }
+size_t paged_prefill_tc_workspace(const PagedView &kv, size_t n_heads, size_t n) { return pp_workspace(pp_tc_most(kv, n_heads, n), kv, n_heads, n); }
 
 int32_t launch_paged_prefill_tc(const PagedView &kv, int type, const void *q, int q_type, size_t n_heads, const int32_t *starts, size_t n_tokens, float scale,
                                 PagedMask mask, void *out, void *ws, cudaStream_t st) {
-    PpParams p = pp_params(kv, mask, q, n_heads, starts, n_tokens, scale, out, ws, pp_tc_grid(kv, n_heads, n_tokens));
+    const int np = q_type == type ? 1 : type == CERA_TYPE_F16 ? 2 : 3;
+    uint32_t splits = pp_tc_splits(kv, n_heads, n_tokens, np, mask);
+    if (mask.window) splits = std::min(splits, pp_tc_splits(kv, n_heads, n_tokens, np, PagedMask{0, 0}));  // which the workspace has room for
+    const PpGrid g = {(uint32_t)pp_units(kv, n_heads, n_tokens, (kv.dim <= 128 ? 2 : 1) * PP_ROWS), splits};
+    PpParams p = pp_params(kv, mask, q, n_heads, starts, n_tokens, scale, out, ws, g);
     auto go = [&](auto cache, auto query) {
         using T = decltype(cache);
         using TQ = decltype(query);
-        if (kv.dim <= 64) return pp_launch<T, TQ, 64>(p, type, st);
-        if (kv.dim <= 128) return pp_launch<T, TQ, 128>(p, type, st);
-        return pp_launch<T, TQ, 256>(p, type, st);
+        if (kv.dim <= 64) return pp_launch<T, TQ, 64>(p, g, type, st);
+        if (kv.dim <= 128) return pp_launch<T, TQ, 128>(p, g, type, st);
+        return pp_launch<T, TQ, 256>(p, g, type, st);
     };
     if (type == CERA_TYPE_F16) return q_type == type ? go(__half(), __half()) : go(__half(), float());
     return q_type == type ? go(__nv_bfloat16(), __nv_bfloat16()) : go(__nv_bfloat16(), float());

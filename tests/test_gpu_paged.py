@@ -200,6 +200,16 @@ def test_prefill_f32_over_many_slots(dtype, dim, growing):
         assert float((got[:, h].double() - want).norm() / want.norm()) < (2.2e-4 if growing else 2e-5)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("window,sink", [(0, 0), (300, 4)])
+def test_prefill_split_keys_of_several_sequences(types, window, sink):
+    """Keys split by the capacity, which most sequences stay far below: parts without keys, and rows that see some of them only."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([2100, 40, 700, 1, 0], 2, 64, 32, types[1], seed=12)
+    _prefill_case(cb, c, 6, types[0], [9, 7, 30, 1, 0], window, sink)
+
+
 def test_prefill_of_more_tokens_than_are_cached():
     """Queries whose place is before the first slot see nothing."""
     need_gpu()
