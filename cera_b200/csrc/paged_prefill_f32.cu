@@ -1,10 +1,12 @@
 // Causal attention of ragged prompt portions over a paged f32 cache, in f32 on the CUDA cores.
 //
-// A row is (token, query head of a KV head).  A CTA of 128 threads owns 64 rows of one (sequence, KV head) and walks tiles of 64 keys with a running maximum and
-// sum: a thread forms the scores of 8 rows x 4 keys, two dimensions an FMA, then 8 rows x 4 (8, 16) dimensions of the result, the weights
-// passing through shared memory in between.  Sixteen lanes share a row's keys and dimensions, so what is read from shared memory is mostly one
-// address for many lanes: 12 loads of 16 bytes for 64 packed FMAs.  The keys of the next tile arrive during softmax and values, its values
-// during the scores.
+// A row is (token, query head of a KV head).  A CTA of 256 threads owns 64 rows of one (sequence, KV head) and walks tiles of 64 keys with a running maximum and
+// sum: a thread forms the scores of 4 rows x 4 keys, two dimensions an FMA, then 4 rows x 4 (8, 16) dimensions of the result, the weights
+// passing through shared memory in between.  Sixteen lanes share a row's keys and dimensions.  The keys of the next tile arrive during softmax and values, its
+// values during the scores.
+//
+// What bounds it: loads from shared memory, 8 of 16 bytes for 32 packed FMAs, at 128 bytes a cycle of an SM (300 tokens of 32 heads over 2300 slots: 398 us, 27 TFLOP/s).  Threads of 8
+// rows x 4 keys load less, 12 for 64, but half as many warps wait for them one by one: 458 us.
 //
 // A row that ends without finite values - a weight of zero times an infinite value of a key it does not see - or that has met no weight is computed again by
 // paged_attend_row, which reads nothing that the row does not see.  Few rows over a long cache: the keys are split over gridDim.z.
@@ -15,7 +17,7 @@ namespace cera {
 
 namespace {
 
-constexpr int PF_ROWS = 64, PF_KT = 64, PF_THREADS = 128;
+constexpr int PF_ROWS = 64, PF_KT = 64, PF_EACH = 4, PF_THREADS = 16 * PF_ROWS / PF_EACH;  // rows of a thread
 
 template <int DP>
 struct Pf {
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
     __shared__ uint32_t there_s[2][2];  // which of a tile's keys there are, of two tiles
     pdl_trigger();
     pdl_wait();
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, dim = p.kv.dim, g16 = lane & 15, r0 = (warp * 2 + (lane >> 4)) * 8;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, dim = p.kv.dim, g16 = lane & 15, r0 = (warp * 2 + (lane >> 4)) * PF_EACH;
     if (warp == 0) {
         PpWork w;
         if (pp_find<PF_ROWS>(p, w, blockIdx.x)) pp_set<PF_ROWS, PF_ROWS, PF_KT>(p, w);
@@ -86,15 +88,15 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
     __syncthreads();
     if (w.x0 < w.x1) copy(off_k, p.kv.k, ks, C::LD);
 
-    int32_t pos[8];
+    int32_t pos[PF_EACH];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) pos[r] = w.row0 + r0 + r < w.rows ? w.slot_of(w.row0 + r0 + r, p.group) : -1;
+    for (int r = 0; r < PF_EACH; ++r) pos[r] = w.row0 + r0 + r < w.rows ? w.slot_of(w.row0 + r0 + r, p.group) : -1;
     const int32_t lo = w.lo0, hi = w.hi0, first_hi = hi >= 0 ? (int32_t)paged_first(p.mask, (uint32_t)hi) : 0;
     const float scale = p.scale * PAGED_LOG2E;
-    float m[8], l[8];
-    float4 acc[8][C::NV];
+    float m[PF_EACH], l[PF_EACH];
+    float4 acc[PF_EACH][C::NV];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < PF_EACH; ++r) {
         m[r] = PP_FLOOR;
         l[r] = 0.0f;
 #pragma unroll
@@ -107,9 +109,9 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
         __syncthreads();  // the keys are there, and the offsets are read
         const uint32_t there[2] = {there_s[x & 1][0], there_s[x & 1][1]};
         if (x + 1 < w.x1) look(x + 1);
-        float2 s2[8][4];
+        float2 s2[PF_EACH][4];
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < PF_EACH; ++r)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s2[r][k] = make_float2(0.0f, 0.0f);
 #pragma unroll 2
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
 #pragma unroll
             for (int k = 0; k < 4; ++k) kk[k] = *reinterpret_cast<const float4 *>(ks + (g16 + 16 * k) * C::LD + d);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
+            for (int r = 0; r < PF_EACH; ++r) {
                 const float4 q = *reinterpret_cast<const float4 *>(qs + (r0 + r) * C::LD + d);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
         else pf_commit();
         const bool all = (there[0] & there[1]) == 0xffffffffu && (int32_t)(slot0 + PF_KT) <= lo + 1 && ((int32_t)slot0 >= first_hi || slot0 + PF_KT <= p.mask.sink);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < PF_EACH; ++r) {
             float z[4], mx = -INFINITY;
             const int32_t first = all || pos[r] < 0 ? 0 : (int32_t)paged_first(p.mask, (uint32_t)pos[r]);
 #pragma unroll
@@ -165,16 +167,16 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
         __syncthreads();  // the values are there (and the weights, which a warp keeps to itself)
 #pragma unroll 2
         for (uint32_t k = 0; k < PF_KT; k += 4) {
-            float4 e[8];
+            float4 e[PF_EACH];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) e[r] = *reinterpret_cast<const float4 *>(ps + (r0 + r) * C::LP + k);
+            for (int r = 0; r < PF_EACH; ++r) e[r] = *reinterpret_cast<const float4 *>(ps + (r0 + r) * C::LP + k);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                 for (int i = 0; i < C::NV; ++i) {
                     const float4 v = *reinterpret_cast<const float4 *>(vs + (k + kk) * DP + (g16 + 16 * i) * 4);
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
+                    for (int r = 0; r < PF_EACH; ++r) {
                         const float wt = kk == 0 ? e[r].x : kk == 1 ? e[r].y : kk == 2 ? e[r].z : e[r].w;
                         const float2 a = __ffma2_rn(make_float2(wt, wt), make_float2(v.x, v.y), make_float2(acc[r][i].x, acc[r][i].y));
                         const float2 b = __ffma2_rn(make_float2(wt, wt), make_float2(v.z, v.w), make_float2(acc[r][i].z, acc[r][i].w));
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
     pf_wait<0>();
     uint32_t again = 0;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < PF_EACH; ++r) {
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
         const uint32_t row = w.row0 + r0 + r;
@@ -211,10 +213,10 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
             *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out) + place * dim + (g16 + 16 * i) * 4) = pos[r] >= 0 ? o : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         const uint32_t bad = __ballot_sync(0xffffffffu, pos[r] >= 0 && check != 0.0f);
-        again |= (bad & 0xffffu ? 1u << r : 0) | (bad >> 16 ? 256u << r : 0);
+        again |= (bad & 0xffffu ? 1u << r : 0) | (bad >> 16 ? 1u << (PF_EACH + r) : 0);
     }
     for (; again; again &= again - 1) {
-        const uint32_t row = w.row0 + warp * 16 + __ffs(again) - 1;
+        const uint32_t row = w.row0 + warp * 2 * PF_EACH + __ffs(again) - 1;
         const size_t place = ((size_t)(w.t0 + row / p.group) * p.heads + h * p.group + row % p.group) * dim;
         __syncwarp();
         paged_attend_row<float, float>(p.kv, p.mask, w.s, h, (uint32_t)w.slot_of(row, p.group), reinterpret_cast<const float *>(p.q) + place, p.scale,
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
 }
 
 uint32_t pf_splits(const PagedView &kv, size_t n_heads, size_t n, PagedMask mask) {
-    return pp_splits(kv, n_heads, n, PF_ROWS, pp_units(kv, n_heads, n, PF_ROWS), PpCost{0.08f * kv.dim, 8.0f}, mask);
+    return pp_splits(kv, n_heads, n, PF_ROWS, pp_units(kv, n_heads, n, PF_ROWS), PpCost{0.065f * kv.dim, 8.0f}, mask);
 }
 
 template <int DP>
