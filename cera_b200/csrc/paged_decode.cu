@@ -6,7 +6,7 @@
 // last unit are shared with others.  What a CTA knows of a shared unit (maximum, sum, weighted values) goes to the workspace, whose size
 // therefore does not depend on the lengths; paged_join_kernel adds the parts up in their order, so a call's bits do not depend on timing.
 //
-// Two warps of a CTA load, keys and values, into a ring of tiles in shared memory: by TMA where a page holds whole groups of a warp's keys, a box of
+// Two warps of a CTA load, keys and values, into a ring of tiles in shared memory: by TMA where a page holds whole groups of eight slots, a box of
 // slots an instruction (a copy for every row, by cp.async or in bulk, took most of what the kernel issued), row by row otherwise.  Four warps
 // compute, each on its own keys of a tile - 16 of 64 over a 16-bit cache, 8 of 32 over f32 - with a running maximum, sum and weighted values of
 // its own; they meet at a unit's end only.  The maximum is raised when a score has passed it by 2^8 (a vote, no exchange), to which the weights'
@@ -848,7 +848,7 @@ int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, 
     const uint32_t G = (uint32_t)std::min<size_t>(DP <= 128 ? pd_grid() : pd_grid() / 2, std::max<size_t>(tiles, 1));  // what fits the SMs at once
     CUtensorMap mk, mv;
     p.box = W::TILE;
-    CERA_TRY(paged_maps(p.kv, type, W::KG, &p.box, &mk, &mv));
+    CERA_TRY(paged_maps(p.kv, type, 8, &p.box, &mk, &mv));
     const bool by_tma = p.box != 0;
     if (!by_tma) p.box = W::TILE;
     auto kernel = by_tma ? paged_decode_kernel<T, TQ, DP, ST, R, true> : paged_decode_kernel<T, TQ, DP, ST, R, false>;

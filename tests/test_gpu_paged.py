@@ -54,7 +54,7 @@ def test_decode_window(types, window, sink):
     _decode_case(cb, R.Cache([1, 2, 0, 17, 100, 300, 41], 2, 64, 16, types[1], seed=window), 6, types[0], window, sink)
 
 
-@pytest.mark.parametrize("page", [1, 3, 16, 24, 64, 1000])
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 64, 1000])
 @pytest.mark.parametrize("layout", ["rows", "interleaved", "heads first"])
 def test_decode_layouts(page, layout):
     need_gpu()
