@@ -11,7 +11,7 @@
 // f32 queries over a 16-bit cache: the query and the weights enter as sums of NP parts of the cache's type (two f16, 22 bits; three
 // bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.  The tensor cores cut a sum at every step instead of rounding it, which
 // a long row would show (5500 slots in one sum: 4.7e-6 off for f16 and 6.6e-6 for bf16, 1.5e-6 with torch's f32 products): the least parts of the queries come first, and after
-// 128 slots O is added to an f32 sum and begun anew (8.7e-7 and 8.9e-7; 1500 queries of 32 heads over them 329 -> 353 us and 587 -> 576).  That sum is in TMEM as far as there is room:
+// 128 slots O is added to an f32 sum and begun anew (8.7e-7 and 8.9e-7; 1500 queries of 32 heads over them, unsplit, 329 -> 353 us and 587 -> 576).  That sum is in TMEM as far as there is room:
 // all of it in local memory takes 536 and 709 us, whose bytes all come from L2.
 //
 // Few rows over a long cache: the keys are split over gridDim.z CTAs and paged_prefill_join_kernel adds the parts up.
@@ -304,50 +304,65 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
     for (uint32_t t = 0; t < C::MT; ++t) tc_commit(&b->o_full[t], me);
 }
 
-// A tile's queries into shared memory, a thread a row -> the factor of its scores, in units of ln 2.
+// A tile's queries into shared memory -> the factor of the lane's row's scores, in units of ln 2.  f32: by warps, a row's pieces of 16 bytes a lane each (a thread a row, whose lines do
+// not stay in what shared memory leaves of L1, takes 37 us for a prompt of 512, this 32).  Others: a thread a row (8000 tokens through a window of 4096 in 473 us, by warps 487).
 template <typename T, typename TQ, int DP, int NP>
 __device__ __forceinline__ float pp_queries(const PpParams &p, const PpWork &w, uint32_t row, uint8_t *to, uint32_t r) {
     using C = Pp<DP, NP>;
+    constexpr int U = 4, L = DP == 256 ? 2 : 1;  // rows at once, loads of a lane
+    const uint32_t lane = r & 31, pieces = p.kv.dim * (uint32_t)sizeof(TQ) / 16;
     const bool live = row < w.rows;
-    const TQ *q = reinterpret_cast<const TQ *>(p.q) + ((size_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group) * p.kv.dim;
+    const uint64_t mine = live ? ((uint64_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group) * p.kv.dim : ~0ull;
     float factor = fmaxf(fabsf(p.scale) * PAGED_LOG2E, 1.2e-38f);  // at a scale of zero all weights are alike, but for those of minus infinity
     const bool turn = p.scale < 0.0f;
     if (NP == 1) {
         const uint32_t flip = turn ? 0x80008000u : 0;
-        for (uint32_t c = 0; c < p.kv.dim / 8; ++c) {
-            uint4 v = live ? reinterpret_cast<const uint4 *>(q)[c] : make_uint4(0, 0, 0, 0);
-            v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-            *reinterpret_cast<uint4 *>(to + (c >> 3) * C::QBLOCK + r * 128 + ((c & 7) ^ (r & 7)) * 16) = v;
+        for (uint32_t c0 = 0; c0 < pieces; c0 += 4) {
+            uint4 v[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) v[i] = live ? reinterpret_cast<const uint4 *>(reinterpret_cast<const TQ *>(p.q) + mine)[c0 + i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t c = c0 + i;
+                *reinterpret_cast<uint4 *>(to + (c >> 3) * C::QBLOCK + r * 128 + ((c & 7) ^ (r & 7)) * 16) = make_uint4(v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
+            }
         }
         return factor;
     }
-    float mul = turn ? -1.0f : 1.0f;
-    if (std::is_same<T, __half>::value) {
-        float most = 0.0f;
-        for (uint32_t c = 0; c < p.kv.dim / 4 && live; ++c) {
-            const float4 v = reinterpret_cast<const float4 *>(q)[c];
-            most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    for (uint32_t i0 = 0; i0 < 32; i0 += U) {
+        uint4 v[U][L];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t at = __shfl_sync(0xffffffffu, mine, i0 + u);
+#pragma unroll
+            for (int k = 0; k < L; ++k)
+                v[u][k] = at != ~0ull && lane + 32 * k < pieces ? reinterpret_cast<const uint4 *>(reinterpret_cast<const TQ *>(p.q) + at)[lane + 32 * k] : make_uint4(0, 0, 0, 0);
         }
-        const int e = most > 0.0f && most <= 3.4e38f ? min(max((int)(__float_as_uint(most) >> 23 & 255) - 127, -120), 120) : 0;
-        mul *= __uint_as_float((uint32_t)(127 - e) << 23);
-        factor *= __uint_as_float((uint32_t)(127 + e) << 23);
-    }
-    for (uint32_t c = 0; c < p.kv.dim / 8; ++c) {
-        float x[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4 v = live ? reinterpret_cast<const float4 *>(q)[2 * c + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            x[4 * i] = v.x * mul;
-            x[4 * i + 1] = v.y * mul;
-            x[4 * i + 2] = v.z * mul;
-            x[4 * i + 3] = v.w * mul;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t rr = r - lane + i0 + u;
+            float mul = turn ? -1.0f : 1.0f;
+            if (std::is_same<T, __half>::value) {
+                uint32_t most = 0;  // of absolute values, whose bits are in their order
+#pragma unroll
+                for (int k = 0; k < L; ++k) most = max(max(max(most, v[u][k].x & 0x7fffffffu), max(v[u][k].y & 0x7fffffffu, v[u][k].z & 0x7fffffffu)), v[u][k].w & 0x7fffffffu);
+                most = __reduce_max_sync(0xffffffffu, most);
+                const int e = most && most < 0x7f800000u ? min(max((int)(most >> 23) - 127, -120), 120) : 0;
+                mul *= __uint_as_float((uint32_t)(127 - e) << 23);
+                if (lane == i0 + u) factor *= __uint_as_float((uint32_t)(127 + e) << 23);
+            }
+#pragma unroll
+            for (int k = 0; k < L; ++k) {
+                const uint32_t c = lane + 32 * k;
+                if (c >= pieces) break;
+                uint32_t lo[NP], hi[NP];
+                pp_parts<T, NP>(__uint_as_float(v[u][k].x) * mul, __uint_as_float(v[u][k].y) * mul, lo);
+                pp_parts<T, NP>(__uint_as_float(v[u][k].z) * mul, __uint_as_float(v[u][k].w) * mul, hi);
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+                    *reinterpret_cast<uint2 *>(to + n * C::QPART + (c >> 4) * C::QBLOCK + rr * 128 + ((c >> 1 & 7) ^ (rr & 7)) * 16 + (c & 1) * 8) = make_uint2(lo[n], hi[n]);
+            }
         }
-        uint32_t u[4][NP];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pp_parts<T, NP>(x[2 * i], x[2 * i + 1], u[i]);
-#pragma unroll
-        for (int k = 0; k < NP; ++k)
-            *reinterpret_cast<uint4 *>(to + k * C::QPART + (c >> 3) * C::QBLOCK + r * 128 + ((c & 7) ^ (r & 7)) * 16) = make_uint4(u[0][k], u[1][k], u[2][k], u[3][k]);
     }
     return factor;
 }
