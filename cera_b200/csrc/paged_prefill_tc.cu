@@ -8,6 +8,7 @@
 // follow one another in the tensor pipe, so S of the next keys may go where P of these is still being read, and when S is complete O
 // is too: the warpgroup that finds a maximum raised by more than 2^8 rescales O on the spot.
 //
+// With 16-bit queries a weight is rounded to the cache's type for its product (the sum has it unrounded): the result, of 16 bits itself, is 1.3 times as far off as with f32 weights.
 // f32 queries over a 16-bit cache: the query and the weights enter as sums of NP parts of the cache's type (two f16, 22 bits; three
 // bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.  The tensor cores cut a sum at every step instead of rounding it, which
 // a long row would show (5500 slots in one sum: 4.7e-6 off for f16 and 6.6e-6 for bf16, 1.5e-6 with torch's f32 products): the least parts of the queries come first, and after
