@@ -766,6 +766,19 @@ __global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, u
     const uint32_t n = b1 - b0 + 1, lane = tid & 31, warp = tid >> 5;
     const uint32_t head = 2 * b0 + (pd_start(b0, total, parts) < u0);  // of the first CTA it may be the last unit
     auto slot = [&](uint32_t i) { return i ? 2 * (b0 + i) : head; };
+    // a warp takes every fourth part, U at a time; the first are on their way before it is known what they count
+    constexpr int U = 4;
+    float4 x[U][2];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (int v = 0; v < U; ++v)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t i = i0 + v * PD_WARPS, d = lane * 4 + k * 128;
+                if (i < n && d < p.kv.dim) x[v][k] = *reinterpret_cast<const float4 *>(p.part + ((size_t)slot(i) * PD_ROWS + r) * p.kv.dim + d);
+            }
+    };
+    load(warp);
     float m = -INFINITY, l = 0.0f;
     for (uint32_t i = tid; i < n; i += PD_MATH) {
         const float2 v = p.ml[(size_t)slot(i) * PD_ROWS + r];
@@ -777,19 +790,19 @@ __global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, u
     __syncthreads();
     m = fmaxf(fmaxf(max_s[0], max_s[1]), fmaxf(max_s[2], max_s[3]));
     float4 o[2] = {};
-#pragma unroll 4
-    for (uint32_t i = warp; i < n; i += PD_WARPS) {  // a warp a part, the warps' sums in their order
-        const float2 v = share_s[i];
-        const float f = v.x == -INFINITY ? 0.0f : pd_exp2(v.x - m);
-        const float *part = p.part + ((size_t)slot(i) * PD_ROWS + r) * p.kv.dim;
-        if (f == 0.0f) continue;
-        l = fmaf(v.y, f, l);
+    for (uint32_t i0 = warp; i0 < n; i0 += U * PD_WARPS) {
+        if (i0 != warp) load(i0);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (lane * 4 + k * 128 < p.kv.dim) {
-                const float4 a = *reinterpret_cast<const float4 *>(part + lane * 4 + k * 128);
-                o[k] = make_float4(fmaf(a.x, f, o[k].x), fmaf(a.y, f, o[k].y), fmaf(a.z, f, o[k].z), fmaf(a.w, f, o[k].w));
-            }
+        for (int v = 0; v < U; ++v) {
+            const uint32_t i = i0 + v * PD_WARPS;
+            const float2 s2 = i < n ? share_s[i] : make_float2(-INFINITY, 0.0f);
+            const float f = s2.x == -INFINITY ? 0.0f : pd_exp2(s2.x - m);
+            if (f == 0.0f) continue;
+            l = fmaf(s2.y, f, l);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (lane * 4 + k * 128 < p.kv.dim) o[k] = make_float4(fmaf(x[v][k].x, f, o[k].x), fmaf(x[v][k].y, f, o[k].y), fmaf(x[v][k].z, f, o[k].z), fmaf(x[v][k].w, f, o[k].w));
+        }
     }
     if (lane == 0) sum_s[warp] = l;
 #pragma unroll

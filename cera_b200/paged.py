@@ -35,7 +35,8 @@ class PagedKv:
     bfloat16 in any strides of whole 16 bytes (head_dim contiguous; keys and values may be interleaved views of one tensor),
     page_table int32 [n_seqs, max_pages] and seq_lens int32 [n_seqs].  Slot j of sequence s is row j % page_size of page
     page_table[s, j // page_size]; an entry outside [0, n_pages) is a page that is not there, whose slots are not seen.  The calls read the
-    table and the lengths when they run, so both may be changed in place between calls and under a captured graph."""
+    table and the lengths when they run, so both may be changed in place between calls and under a captured graph.  Sequences may share pages
+    (a common beginning) that are only read; what paged_append and paged_evict write must be in pages of one sequence."""
 
     def __init__(self, k_pages, v_pages, page_table, seq_lens):
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("seq_lens", seq_lens)):

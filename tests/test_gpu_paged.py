@@ -554,6 +554,18 @@ def test_pages_past_four_gigabytes(q_dtype, dtype):
     assert (kept == 128).all() and torch.equal(k[pages - 1, 0], k[pages - 3, 0])
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_sequences_that_share_their_beginning(types):
+    """Pages in several tables, and twice in one: what is seen is as if they were copies."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([100, 90, 160], 2, 64, 16, types[1], seed=85)
+    c.table[1, :4] = c.table[0, :4]
+    c.table[2, 5:8] = c.table[2, 1:4]
+    _decode_case(cb, c, 8, types[0], weights=True)
+    _prefill_case(cb, c, 8, types[0], [20, 1, 70])
+
+
 def test_the_same_call_gives_the_same_bits():
     need_gpu()
     import cera_b200 as cb
