@@ -166,7 +166,7 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t x) {  // inclusive
 __device__ __forceinline__ uint32_t low_bits(uint32_t n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
 // A cluster per pair and a slice of its slots per CTA.  Histograms stay where they are counted: every CTA's first warp adds up their sums of 64 bins each, then the 64
-// bins that matter (all bins of four CTAs read by each of them took 3400 clocks, this 1200).  A warp has `wide` <= 64 words of 32 slots of the slice, whose
+// bins that matter (all bins of four CTAs read by each of them took 3400 clocks a round).  A warp has `wide` <= 64 words of 32 slots of the slice, whose
 // kept ones it finds by ballots.  The kept slots past the budget are handed to the gaps by the CTAs that have them, since these are spread evenly.
 template <bool CLUSTER, bool MOVE>
 __global__ void __launch_bounds__(PICK_THREADS) paged_pick_kernel(const PagedView kv, const float *weights, const int32_t *positions, size_t stride, uint32_t budget,
