@@ -8,7 +8,7 @@
 // follow one another in the tensor pipe, so S of the next keys may go where P of these is still being read, and when S is complete O
 // is too: the warpgroup that finds a maximum raised by more than 2^8 rescales O on the spot.
 //
-// With 16-bit queries a weight is rounded to the cache's type for its product (the sum has it unrounded): the result, of 16 bits itself, is 1.3 times as far off as with f32 weights.
+// Weights enter their product as a sum of two parts of the cache's type (f16 22 bits, bf16 16; as one part they put the result, rounded to 16 bits, 1.4 times as far off).
 // f32 queries over a 16-bit cache: the query and the weights enter as sums of NP parts of the cache's type (two f16, 22 bits; three
 // bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.  The tensor cores cut a sum at every step instead of rounding it, which
 // a long row would show (5500 slots in one sum: 4.7e-6 off for f16 and 6.6e-6 for bf16, 1.5e-6 with torch's f32 products): the least parts of the queries come first, and after
@@ -42,11 +42,11 @@ constexpr uint32_t PP_MASKS = 4;  // tiles whose masks are kept: more than the k
 // Shapes by the padded head size and the number of parts.
 template <int DP, int NP>
 struct Pp {
-    static constexpr int MT = DP <= 128 ? 2 : 1;
+    static constexpr int MT = DP <= 128 ? 2 : 1, WP = NP == 1 ? 2 : NP;  // parts of a weight
     static constexpr int KT = NP == 1 ? 128 : DP == 256 && NP == 3 ? 32 : 64;
     static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
     static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
-    static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((NP * P_COLS > KT ? NP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
+    static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((WP * P_COLS > KT ? WP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
     static constexpr uint32_t FLUSH = 128 / KT;  // tiles that O adds up with f32 queries
     static constexpr uint32_t SPARE = (512 - MT * T_COLS) / MT / 32 * 32, KEPT = NP == 1 ? 0 : SPARE < DP ? SPARE : DP;  // numbers of a row's sum that TMEM has room for
     static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 4);  // warpgroups: softmax of a tile each; products, two loaders and a warp of nothing
@@ -55,7 +55,7 @@ struct Pp {
 };
 
 struct PpBars {
-    uint64_t q_full, v_part, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, v_part, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], p_low[2], o_full[2];
 };
 
 __device__ __forceinline__ float pp_max3(float a, float b, float c) {
@@ -287,9 +287,14 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
                 const uint32_t s = tmem + t * C::T_COLS, o = s + C::S_COLS;
                 const uint64_t vd = v0 + st * (C::HALF / 16);
 #pragma unroll 1
-                for (int part = 0; part < NP; ++part)
+                for (int part = 0; part < C::WP; ++part) {
+                    if (NP == 1 && part) {  // the lower parts come while the upper ones are multiplied
+                        if (!arrived(&b->p_low[t], added[t] & 1)) return;
+                        tc_fence_after();
+                    }
 #pragma unroll
                     for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, (NP == 1 ? added[t] : added[t] % C::FLUSH) | part | k, me);
+                }
                 ++added[t];
             }
             if (t + 1 == C::MT) tc_commit(&b->v_empty[st], me);
@@ -453,8 +458,9 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 see[k] &= pp_low(pos + 1 - at) & (~pp_low(first - at) | pp_low(sinks - at));
             }
         }
-        // Weights for the maximum that is known; where the tile has a score past it by more than 2^8, O and the
-        // sum are rescaled and the weights, whose scores are still in registers, formed again.
+        // f32 queries: weights for the maximum that is known; where the tile has a score past it by more than 2^8, O and the
+        // sum are rescaled and the weights, whose scores are still in registers, formed again.  16-bit queries: the maximum first, then the weights' upper parts, which take
+        // the place of the scores, and the lower parts beside the upper ones' product (all of a weight at once: 752 us for 8000 tokens through a window of 4096, 615 so).
         constexpr int Q = C::KT / 32;
         uint32_t v[Q][32];
 #pragma unroll
@@ -474,6 +480,10 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 pp_parts<T, NP>(x.x, x.y, u);
 #pragma unroll
                 for (int n = 0; n < NP; ++n) wd[n][e] = u[n];
+                if (NP == 1) {
+                    v[j][2 * e] = __float_as_uint(x.x);
+                    v[j][2 * e + 1] = __float_as_uint(x.y);
+                }
             }
 #pragma unroll
             for (int n = 0; n < NP; ++n) tmem_st16(ts + n * C::P_COLS + 16 * j, wd[n]);
@@ -490,7 +500,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
                 for (int e = 0; e < 32; e += 8)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top[i] = pp_max3(top[i], __uint_as_float(v[j][e + 2 * i]), __uint_as_float(v[j][e + 2 * i + 1]));
-                form(j);
+                if (NP > 1) form(j);
             }
         };
         if (all) stream(std::true_type());
@@ -516,6 +526,12 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             }
             base = make_float2(PP_LIFT - m, PP_LIFT - m);
             sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+            if (NP > 1) {
+#pragma unroll
+                for (int j = 0; j < Q; ++j) form(j);
+            }
+        }
+        if (NP == 1) {
 #pragma unroll
             for (int j = 0; j < Q; ++j) form(j);
         }
@@ -524,6 +540,23 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
         tc_fence_before();
         __syncwarp();
         if (lane == 0) tma::mbar_arrive(&b->p_full[t]);
+        if (NP == 1) {
+#pragma unroll
+            for (int j = 0; j < Q; ++j) {
+                uint32_t wd[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    uint32_t u[2];
+                    pp_parts<T, 2>(__uint_as_float(v[j][2 * e]), __uint_as_float(v[j][2 * e + 1]), u);
+                    wd[e] = u[1];
+                }
+                tmem_st16(ts + C::P_COLS + 16 * j, wd);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tma::mbar_arrive(&b->p_low[t]);
+        }
         ++done;
     }
     if (ok && done) ok = tma::mbar_wait_warp(&b->o_full[t], 0, abort_flag, status, 4u);
@@ -621,6 +654,7 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
             for (int i = 0; i < 2; ++i) {
                 tma::mbar_init(&bars.s_full[i], 1);
                 tma::mbar_init(&bars.p_full[i], 4);
+                tma::mbar_init(&bars.p_low[i], 4);
                 tma::mbar_init(&bars.o_full[i], 1);
             }
             tma::mbar_init_fence();
@@ -661,7 +695,7 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
 // np: parts of a query.
 uint32_t pp_tc_splits(const PagedView &kv, size_t n_heads, size_t n, int np, PagedMask mask) {
     const size_t rows = (kv.dim <= 128 ? 2 : 1) * PP_ROWS;
-    const PpCost cost = {(np == 1 ? 1.05f : np == 2 ? 2.3f : 3.7f) * kv.dim / 128, np == 1 ? 9.0f : 14.0f};
+    const PpCost cost = {(np == 1 ? 1.3f : np == 2 ? 2.3f : 3.7f) * kv.dim / 128, np == 1 ? 9.0f : 14.0f};
     return pp_splits(kv, n_heads, n, rows, pp_units(kv, n_heads, n, rows), cost, mask);
 }
 // With any queries and mask.

@@ -1,0 +1,37 @@
+"""The paged cache's operators where they are easily wrong: bits of weights, sums of very many slots, scores and scales that are not ordinary numbers, a result over its
+queries, and forms that only larger groups or several sequences reach."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as R
+from gpu_util import need_gpu
+from test_gpu_paged import TYPES, _decode_case, _evict_case, _q, _track
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---- prompts of 16 bits ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("dim,length,new,window", [(64, 40, 40, 9), (128, 310, 300, 9), (256, 12, 7, 0), (96, 3000, 2, 11)])
+def test_weights_of_16_bit_prompts_keep_more_bits_than_the_result(dtype, dim, length, new, window):
+    """Few slots with weights that are nearly alike, and values that nearly cancel.  Bound: what f32 arithmetic may be off by, weights in two parts of the type (f16 2^-21,
+    which R.tolerance has; bf16 2^-8 of 2^-8), the result rounded once.  A weight rounded once would be off by 2^-11 or 2^-8."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([length], 2, dim, 16, dtype, seed=dim)
+    q = _q(new, 6, dim, dtype, size=0.2)
+    scale = 1.0 / math.sqrt(dim)
+    got = cb.paged_prefill_attention(c.cuda(), q.cuda(), _i32([0, new]), scale, window=window)
+    for i in range(new):
+        want, pv, size, js, _ = R.attend(c, 0, length - new + i, q[i], scale, window)
+        f32 = R.tolerance(want, pv, size, len(js), dim, F32, dtype) + (2.0 ** -16 * pv if dtype == BF16 else 0.0)
+        R.check(got[i], want, f32 + torch.finfo(dtype).eps / 2 * (want.abs() + f32) + 2.0 ** -24, f"query {i}")
