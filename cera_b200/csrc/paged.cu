@@ -97,6 +97,12 @@ int32_t check_heads(const char *what, const PagedView &v, int32_t type, int32_t 
     return CERA_CUDA_OK;
 }
 
+// Rows (token, head of a KV head) are counted in 31 bits.
+int32_t check_tokens(const char *what, const PagedView &v, size_t n_heads, size_t n_tokens) {
+    if (n_tokens > 0x7fffffffu / (n_heads / v.hk)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: %zu tokens", what, n_tokens);
+    return CERA_CUDA_OK;
+}
+
 int32_t check_workspace(const char *what, const void *ws, size_t have, size_t need) {
     if (have < need || (need && !ws) || ((uintptr_t)ws & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: a workspace of %zu bytes (%zu, on a 16-byte boundary)", what, have, need);
     return CERA_CUDA_OK;
@@ -193,7 +199,10 @@ int32_t cera_cuda_paged_decode_attention(const cera_cuda_paged_kv *kv, const voi
 
 size_t cera_cuda_paged_prefill_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads, size_t n_tokens) {
     PagedView v;
-    if (view("paged_prefill_attention", kv, &v) != CERA_CUDA_OK || check_heads("paged_prefill_attention", v, kv->type, kv->type, n_heads) != CERA_CUDA_OK) return 0;
+    if (view("paged_prefill_attention", kv, &v) != CERA_CUDA_OK || check_heads("paged_prefill_attention", v, kv->type, kv->type, n_heads) != CERA_CUDA_OK ||
+        check_tokens("paged_prefill_attention", v, n_heads, n_tokens) != CERA_CUDA_OK)
+        return 0;
+    if (n_tokens == 0 || v.n_seqs == 0) return 16;  // nothing to do, which is no refusal
     return paged_prefill_workspace(v, kv->type, n_heads, n_tokens);
 }
 
@@ -204,9 +213,9 @@ int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const vo
     PagedView v;
     CERA_TRY(view(what, kv, &v));
     CERA_TRY(check_heads(what, v, kv->type, q_type, n_heads));
+    CERA_TRY(check_tokens(what, v, n_heads, n_tokens));
     if (n_tokens == 0 || v.n_seqs == 0) return CERA_CUDA_OK;
     if (!starts_dev) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: no starts", what);
-    if (n_tokens * (n_heads / v.hk) > 0x7fffffffu) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: %zu tokens", what, n_tokens);
     if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: queries or result null or off a 16-byte boundary", what);
     CERA_TRY(check_workspace(what, workspace_dev, workspace_bytes, paged_prefill_workspace(v, kv->type, n_heads, n_tokens)));
     return launch_paged_prefill(v, kv->type, q_dev, q_type, n_heads, starts_dev, n_tokens, scale, PagedMask{window, n_sink}, out_dev, workspace_dev,

@@ -35,3 +35,18 @@ def test_weights_of_16_bit_prompts_keep_more_bits_than_the_result(dtype, dim, le
         want, pv, size, js, _ = R.attend(c, 0, length - new + i, q[i], scale, window)
         f32 = R.tolerance(want, pv, size, len(js), dim, F32, dtype) + (2.0 ** -16 * pv if dtype == BF16 else 0.0)
         R.check(got[i], want, f32 + torch.finfo(dtype).eps / 2 * (want.abs() + f32) + 2.0 ** -24, f"query {i}")
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_a_step_without_tokens(types):
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([20, 3], 2, 64, 16, types[1], seed=3)
+    cache = c.cuda()
+    q = torch.empty(0, 4, 64, dtype=types[0], device="cuda")
+    assert cb.paged_prefill_attention(cache, q, _i32([0, 0, 0]), 0.125).shape == (0, 4, 64)
+    cb.paged_append(cache, torch.empty(0, 2, 64, dtype=types[0], device="cuda"), torch.empty(0, 2, 64, dtype=types[0], device="cuda"), _i32([0, 0, 0]))
+    none = cb.PagedKv(cache.k_pages, cache.v_pages, cache.page_table[:0], cache.seq_lens[:0])
+    assert cb.paged_decode_attention(none, q, 0.125).shape == (0, 4, 64)
+    assert cb.paged_prefill_attention(none, q, _i32([0]), 0.125).shape == (0, 4, 64)
+    assert torch.equal(c.kd.cpu().view(torch.uint8), c.k.contiguous().view(torch.uint8))
