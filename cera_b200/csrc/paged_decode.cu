@@ -15,7 +15,9 @@
 // 16-bit cache: mma.sync, 16 rows = eight heads twice: the upper half of each query and weight as the type has it, and what that leaves,
 // so an f32 query or weight counts with 22 bits (f16) in the same instructions; bf16's 16 bits are too few for an f32 query, whose third
 // part takes a second product.  An f16 part is scaled by a power of two per query, weights by 2^7, so that what f16 cannot tell from zero is 2^-32
-// of the largest weight.
+// of the largest weight.  The tensor cores cut a sum at every step instead of rounding it (one sum a unit: 5.4e-5 off at 40 960 slots, 1.6e-4 at 131 072), so after JOIN tiles a
+// warp's sums are added in f32 to those it keeps in shared memory, and begun anew: eight tiles where the result has 32 bits (4.4e-7 off at 40 960 slots; sixteen 1.1e-6), 64 where it has 16 (5.6e-6
+// beside its rounding; eight would cost 24 conversations 1.5 us of 39).
 // f32 cache: FMAs, four lanes a key for the scores, a lane 4 dimensions of every head for the values.
 //
 // With weights wanted the scaled scores are stored on the way (4 bytes a head and slot, beside the 2 dim that are read for it), and
@@ -166,9 +168,30 @@ template <typename T, typename TQ, int DP>
 struct PdMma {
     static constexpr int KG = 16, ROWS = PD_ROWS, TILE = PD_WARPS * KG, BLOCK = 64;  // BLOCK: numbers of a 128-byte row
     static constexpr bool SPLIT = sizeof(TQ) == 4, BF = sizeof(T) == 2 && !std::is_same<T, __half>::value, THIRD = SPLIT && BF;
+    static constexpr uint32_t JOIN = SPLIT ? 8 : 64;  // a power of two
     uint32_t qf[DP / 16][SPLIT ? 4 : 2], q3[THIRD ? DP / 16 : 1][2];
     uint32_t wf[4], w3[4];
     float acc[DP / 8][4], m, l, factor;
+    float *kept;  // this lane's numbers of the warp's sums [8][dim] in shared memory
+    bool some;    // there are such sums
+
+    // the value of column pair n that acc has, number i: of an infinite value the weight's upper part says it all
+    __device__ __forceinline__ float value(int n, int i) const {
+        const float hi = acc[n][i], both = hi + acc[n][i + 2];
+        return fabsf(both) < INFINITY ? both : hi;
+    }
+    __device__ __forceinline__ void keep(const PdParams &p) {
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+            if (n * 8 < p.kv.dim) {
+                float2 *to = reinterpret_cast<float2 *>(kept + n * 8);
+                const float2 old = some ? *to : make_float2(0.0f, 0.0f);
+                *to = make_float2(old.x + value(n, 0), old.y + value(n, 1));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+            }
+        some = true;
+    }
 
     static __device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo) {
         if (BF) split_bf16(x, y, hi, lo);
@@ -189,8 +212,10 @@ struct PdMma {
         return a;
     }
 
-    __device__ __forceinline__ void begin(const PdParams &p, uint32_t s, uint32_t head0, uint32_t rows, float *) {
+    __device__ __forceinline__ void begin(const PdParams &p, uint32_t s, uint32_t head0, uint32_t rows, float *, float *sums) {
         const uint32_t lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+        kept = sums + r * p.kv.dim + 2 * c;
+        some = false;
         const TQ *q = reinterpret_cast<const TQ *>(p.q) + ((size_t)s * p.heads + head0 + r) * p.kv.dim + 2 * c;
         const bool live = r < rows;
         factor = p.scale * PAGED_LOG2E;
@@ -289,6 +314,11 @@ struct PdMma {
                 for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[n][i] *= f;
+                if (some)
+                    for (uint32_t n = 0; n < p.kv.dim; n += 8) {
+                        float2 *to = reinterpret_cast<float2 *>(kept + n);
+                        *to = make_float2(to->x * f, to->y * f);
+                    }
             }
         }
         const float base = PD_LIFT - m;
@@ -329,20 +359,15 @@ struct PdMma {
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if ((lane & 3) == 0) ml[lane >> 2] = make_float2(m, l);
     }
-    // the weighted values for the maxima `all` of each row, [8][dim]
-    __device__ __forceinline__ void values(const PdParams &p, const float *all, float *to) const {
-        const uint32_t lane = threadIdx.x & 31, r = lane >> 2;
-        const float f = pd_exp2(m - all[r]);
+    // the weighted values for the maxima `all` of each row, where the sums are kept
+    __device__ __forceinline__ void values(const PdParams &p, const float *all, float *) {
+        const float f = pd_exp2(m - all[(threadIdx.x & 31) >> 2]);
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
             if (n * 8 < p.kv.dim) {
-                float2 o;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float hi = acc[n][i], both = hi + acc[n][i + 2];
-                    (i ? o.y : o.x) = (fabsf(both) < INFINITY ? both : hi) * f;
-                }
-                *reinterpret_cast<float2 *>(to + r * p.kv.dim + n * 8 + 2 * (lane & 3)) = o;
+                float2 *to = reinterpret_cast<float2 *>(kept + n * 8);
+                const float2 old = some ? *to : make_float2(0.0f, 0.0f);
+                *to = make_float2((old.x + value(n, 0)) * f, (old.y + value(n, 1)) * f);
             }
     }
 };
@@ -354,7 +379,9 @@ struct PdFma {
     float4 acc[R][NV];
     float m[NZ], l[NZ];  // of heads NZ (lane % 4) + [0, NZ); l over this lane's keys
 
-    __device__ __forceinline__ void begin(const PdParams &p, uint32_t s, uint32_t head0, uint32_t rows, float *qs) {
+    static constexpr uint32_t JOIN = 1;
+    __device__ __forceinline__ void keep(const PdParams &) {}  // FMAs round
+    __device__ __forceinline__ void begin(const PdParams &p, uint32_t s, uint32_t head0, uint32_t rows, float *qs, float *) {
         const uint32_t lane = threadIdx.x & 31;
         const float *q = reinterpret_cast<const float *>(p.q) + ((size_t)s * p.heads + head0) * p.kv.dim;
         __syncwarp();
@@ -632,7 +659,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
             rows = min(p.group - c * PD_ROWS, (uint32_t)PD_ROWS);
             first_tile = at.tile;
             any = 0;
-            w.begin(p, at.s, head0, rows, qs);
+            w.begin(p, at.s, head0, rows, qs, values + warp * R * p.kv.dim);
         }
         const uint32_t st = x % ST, slot0 = at.slot(at.tile, TILE) + warp * KG;
         const uint8_t *ks = smem + st * S::STAGE;
@@ -661,6 +688,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
         const bool last = at.tile + 1 == at.tiles;
         at.step(line, p.kv, p.mask);
         more = at.behind(end);
+        if (x % W::JOIN == W::JOIN - 1) w.keep(p);
         if (last || !more) {
             // the warps' shares of the unit
             w.end(ml_s[warp]);

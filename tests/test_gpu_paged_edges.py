@@ -50,3 +50,35 @@ def test_a_step_without_tokens(types):
     assert cb.paged_decode_attention(none, q, 0.125).shape == (0, 4, 64)
     assert cb.paged_prefill_attention(none, q, _i32([0]), 0.125).shape == (0, 4, 64)
     assert torch.equal(c.kd.cpu().view(torch.uint8), c.k.contiguous().view(torch.uint8))
+
+
+def _shared(cb, n, slots, heads, dim, dtype, page=64):
+    """n sequences over the same pages, values of one sign -> cache, keys and values [slots][heads][dim]."""
+    g = torch.Generator("cuda").manual_seed(dim)
+    k = torch.randn(slots // page, page, heads, dim, generator=g, device="cuda").to(dtype)
+    v = (torch.rand(slots // page, page, heads, dim, generator=g, device="cuda") + 0.5).to(dtype)
+    table = torch.arange(slots // page, dtype=torch.int32, device="cuda").expand(n, -1).contiguous()
+    return cb.PagedKv(k, v, table, _i32([slots] * n)), k.reshape(slots, heads, dim), v.reshape(slots, heads, dim)
+
+
+# ---- one token each -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("slots", [40960, 131072])
+def test_decode_over_very_many_slots(types, slots):
+    """64 sequences of 8 heads, so that a CTA has whole units.  Bound, relative to the result's norm: 8 steps (16 with a third part) that the tensor cores cut by 2^-23 at most, 1.9e-6; the
+    sums of those, and of the weights, in f32: up to 2048 roundings of 2^-25 at random signs, 1.4e-6; scores of size 0.05, exponentials and parts 2^-20, 1e-6.  16-bit queries: every number, 64 steps
+    (7.6e-6), sums of those in f32, weights in two parts (bf16 2^-16) and the rounding of the result.  (A unit in one sum: 5.4e-5 at 40 960 slots, 1.6e-4 at 131 072.)"""
+    need_gpu()
+    import cera_b200 as cb
+    dim = 128
+    cache, k, v = _shared(cb, 64, slots, 8, dim, types[1])
+    q = (torch.randn(64, 8, dim, generator=torch.Generator("cuda").manual_seed(1), device="cuda") * 0.01).to(types[0])
+    got = cb.paged_decode_attention(cache, q, 1.0 / math.sqrt(dim))
+    for h in (0, 5):
+        want = torch.softmax(q[:, h].double() @ k[:, h].double().T / math.sqrt(dim), -1) @ v[:, h].double()
+        off = (got[:, h].double() - want).abs()
+        if types[0] == F32:
+            assert float(off.norm() / want.norm()) < 8e-6
+        else:
+            assert float((off / want).max()) < torch.finfo(types[0]).eps / 2 + (2e-5 if types[0] == F16 else 5e-5)
