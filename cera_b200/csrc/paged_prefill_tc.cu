@@ -13,7 +13,8 @@
 // bf16, 24), a product each; f16 parts are scaled by a power of two per row, weights by 2^7.  The tensor cores cut a sum at every step instead of rounding it, which
 // a long row would show (5500 slots in one sum: 4.7e-6 off for f16 and 6.6e-6 for bf16, 1.5e-6 with torch's f32 products): the least parts of the queries come first, and after
 // 128 slots O is added to an f32 sum and begun anew (8.7e-7 and 8.9e-7; 1500 queries of 32 heads over them, unsplit, 329 -> 353 us and 587 -> 576).  That sum is in TMEM as far as there is room:
-// all of it in local memory takes 536 and 709 us, whose bytes all come from L2.
+// all of it in local memory takes 536 and 709 us, whose bytes all come from L2.  With 16-bit queries O is emptied likewise, but seldom
+// (pp_flush; 131 072 slots of one sign in one sum lose 1.5e-4 with weights of one part).
 //
 // Few rows over a long cache: the keys are split over gridDim.z CTAs and paged_prefill_join_kernel adds the parts up.
 //
@@ -47,12 +48,16 @@ struct Pp {
     static constexpr uint32_t QPART = PP_ROWS * DP * 2, QBLOCK = PP_ROWS * 128, KBLOCK = KT * 128, HALF = KT * DP * 2;
     static constexpr int ST = (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF) >= 3 ? 3 : (227 * 1024 - 2048 - MT * NP * (int)QPART) / (2 * (int)HALF);
     static constexpr uint32_t P_COLS = KT / 2, S_COLS = ((WP * P_COLS > KT ? WP * P_COLS : KT) + 31) / 32 * 32, T_COLS = S_COLS + DP;  // TMEM columns of a tile: S or P, then O
-    static constexpr uint32_t FLUSH = 128 / KT;  // tiles that O adds up with f32 queries
     static constexpr uint32_t SPARE = (512 - MT * T_COLS) / MT / 32 * 32, KEPT = NP == 1 ? 0 : SPARE < DP ? SPARE : DP;  // numbers of a row's sum that TMEM has room for
     static constexpr int MATH = 4 * MT, THREADS = 32 * (MATH + 4);  // warpgroups: softmax of a tile each; products, two loaders and a warp of nothing
     static constexpr size_t SMEM = 1024 + (size_t)MT * NP * QPART + (size_t)ST * 2 * HALF;
     static_assert(ST >= 1 && MT * T_COLS <= 512, "does not fit");
 };
+
+// Tiles that O adds up, a power of two.  The tensor cores cut a sum at every step (16 slots of one part): 8192 steps lost 1.5e-4, and a step 2^-23 at most.  With 16-bit queries, whose
+// result is rounded itself, 4096 slots (f16: 512 steps, 6e-5 at most of 4.9e-4) or 32 768 (bf16: 4096 steps, 4.9e-4 of 3.9e-3).
+template <typename T, int DP, int NP>
+constexpr uint32_t pp_flush = (NP > 1 ? 128 : std::is_same<T, __half>::value ? 4096 : 32768) / Pp<DP, NP>::KT;
 
 struct PpBars {
     uint64_t q_full, v_part, k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2], p_low[2], o_full[2];
@@ -241,6 +246,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
                                             unsigned int *status) {
     using C = Pp<DP, NP>;
     constexpr bool BF = !std::is_same<T, __half>::value;
+    constexpr uint32_t FLUSH = pp_flush<T, DP, NP>;
     const uint32_t me = elect_one(), id_s = pp_idesc(BF, C::KT, false), id_o = pp_idesc(BF, p.kv.dim, true), n = w.x1 - w.x0, steps = p.kv.dim / 16;
     const uint64_t q0 = smem_desc_sw128(tma::smem_u32(qs)), k0 = smem_desc_sw128(tma::smem_u32(ks)), v0 = pp_desc_v(tma::smem_u32(vs), C::KBLOCK);  // address fields count 16 bytes
     auto arrived = [&](uint64_t *bar, uint32_t parity) { return tma::mbar_wait_warp(bar, parity, abort_flag, status, 2u); };
@@ -293,7 +299,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
                         tc_fence_after();
                     }
 #pragma unroll
-                    for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, (NP == 1 ? added[t] : added[t] % C::FLUSH) | part | k, me);
+                    for (uint32_t k = 0; k < C::KT / 16; ++k) tc_mma_f16_ts(o, s + part * C::P_COLS + 8 * k, vd + k * (2048 / 16), id_o, added[t] % FLUSH | part | k, me);
                 }
                 ++added[t];
             }
@@ -378,6 +384,7 @@ template <typename T, typename TQ, int DP, int NP>
 __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, uint32_t t, uint8_t *qs, uint32_t tmem, PpBars *b, const uint32_t (*masks)[4],
                                            volatile uint32_t *abort_flag, unsigned int *status) {
     using C = Pp<DP, NP>;
+    constexpr uint32_t FLUSH = pp_flush<T, DP, NP>;
     const uint32_t lane = threadIdx.x & 31, quad = threadIdx.x >> 5 & 3, r = quad * 32 + lane, row = w.row0 + t * PP_ROWS + r;
     const uint32_t ts = tmem + t * C::T_COLS + (quad * 32 << 16), to = ts + C::S_COLS;
     const float c = pp_queries<T, TQ, DP, NP>(p, w, row, qs + t * NP * C::QPART, r);
@@ -394,9 +401,9 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     float m = PP_FLOOR, l = 0.0f;
     uint32_t done = 0;
     bool ok = true;
-    // with f32 queries: the sums of whole groups of FLUSH tiles, the first KEPT numbers in TMEM and the others in local memory
+    // the sums of whole groups of FLUSH tiles, the first KEPT numbers in TMEM and the others in local memory
     const uint32_t ta = tmem + C::MT * C::T_COLS + t * C::KEPT + (quad * 32 << 16);
-    constexpr int FAR = NP == 1 ? 0 : DP - (int)C::KEPT;
+    constexpr int FAR = DP - (int)C::KEPT;
     alignas(16) float far[FAR ? FAR : 1];
     // f(number, its sum) for every number of the row, 32 at a time
     auto sums = [&](auto f) {
@@ -427,13 +434,14 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             for (int e = 0; e < 32; ++e) far[d + e] = __uint_as_float(s[e]);
         }
     };
+    float m_far = PP_FLOOR;  // 16-bit queries: the maximum that `far` stands for
     auto flush = [&] {
         sums([&](uint32_t d, uint32_t (&s)[32]) {
             uint32_t o[32];
             tmem_ld32(to + d, o);
             tmem_wait_ld32(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = done == C::FLUSH ? o[e] : __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(o[e]));
+            for (int e = 0; e < 32; ++e) s[e] = done == FLUSH ? o[e] : __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(o[e]));
         });
     };
     for (uint32_t i = 0; i < w.x1 - w.x0; ++i) {
@@ -442,7 +450,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
         ok = tma::mbar_wait_warp(&b->s_full[t], done & 1, abort_flag, status, 4u);
         if (!ok) break;
         tc_fence_after();
-        if (NP > 1 && done && done % C::FLUSH == 0) flush();  // O is complete up to the tile before, and begins anew
+        if (NP > 1 && done && done % FLUSH == 0) flush();  // O is complete up to the tile before, and begins anew
         // which of the tile's keys this row sees; nothing to look at where every row sees all
         uint32_t see[(C::KT + 31) / 32];
         bool all = (int32_t)(slot0 + C::KT) <= p_lo + 1 && ((int32_t)slot0 >= first_hi || slot0 + C::KT <= p.mask.sink);
@@ -511,7 +519,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             const float f = raise ? pp_exp2(m - mx) : 1.0f;
             if (raise) m = mx;
             l *= f;
-            if (NP > 1 && done >= C::FLUSH)
+            if (NP > 1 && done >= FLUSH)
                 sums([&](uint32_t, uint32_t (&s)[32]) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
@@ -532,6 +540,18 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
             }
         }
         if (NP == 1) {
+            if (done && done % FLUSH == 0) {  // O goes to `far` and begins anew
+                const float f = pp_exp2(m_far - m);
+                m_far = m;
+#pragma unroll 1
+                for (uint32_t d = 0; d < p.kv.dim; d += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(to + d, o);
+                    tmem_wait_ld16(o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) far[NP == 1 ? d + e : 0] = done == FLUSH ? __uint_as_float(o[e]) : fmaf(far[NP == 1 ? d + e : 0], f, __uint_as_float(o[e]));
+                }
+            }
 #pragma unroll
             for (int j = 0; j < Q; ++j) form(j);
         }
@@ -562,7 +582,20 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     if (ok && done) ok = tma::mbar_wait_warp(&b->o_full[t], 0, abort_flag, status, 4u);
     if (!ok) return;
     tc_fence_after();
-    if (NP > 1 && done > C::FLUSH) {  // O joins the sums
+    if (NP == 1 && done > FLUSH) {
+        const float f = pp_exp2(m_far - m);
+#pragma unroll 1
+        for (uint32_t d = 0; d < p.kv.dim; d += 16) {
+            uint32_t o[16];
+            tmem_ld16(to + d, o);
+            tmem_wait_ld16(o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(fmaf(far[NP == 1 ? d + e : 0], f, __uint_as_float(o[e])));
+            tmem_st16(to + d, o);
+        }
+        tmem_wait_st();
+    }
+    if (NP > 1 && done > FLUSH) {  // O joins the sums
         sums([&](uint32_t d, uint32_t (&s)[32]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

@@ -82,3 +82,51 @@ def test_decode_over_very_many_slots(types, slots):
             assert float(off.norm() / want.norm()) < 8e-6
         else:
             assert float((off / want).max()) < torch.finfo(types[0]).eps / 2 + (2e-5 if types[0] == F16 else 5e-5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+def test_16_bit_prompts_over_very_many_slots(dtype):
+    """10 240 queries over 131 072 slots of one sign, unsplit.  Bound: 4096 slots (bf16: 32 768) in one sum are 512 (4096) steps that the tensor cores cut by 2^-23 at most, 6.1e-5
+    (4.9e-4), and 32 of those sums in f32 2e-6; scores of size 0.05 and two parts of a weight 2^-16 (bf16) or 2^-21; the result rounded once.  In one sum with one part a weight 131 072 slots lose
+    1.5e-4 on average, a third of f16's rounding."""
+    need_gpu()
+    import cera_b200 as cb
+    n, slots, dim = 10240, 131072, 64
+    cache, k, v = _shared(cb, 1, slots, 1, dim, dtype)
+    q = (torch.randn(n, 4, dim, generator=torch.Generator("cuda").manual_seed(1), device="cuda") * 0.01).to(dtype)
+    got = cb.paged_prefill_attention(cache, q, _i32([0, n]), 0.125)
+    rows = torch.arange(0, n, 97, device="cuda")
+    hidden = torch.arange(slots, device="cuda") > (slots - n + rows)[:, None]
+    for h in (0, 3):
+        x = (q[rows, h].double() @ k[:, 0].double().T * 0.125).masked_fill_(hidden, -math.inf)
+        want = torch.softmax(x, -1) @ v[:, 0].double()
+        off = (got[rows, h].double() - want).abs() / want
+        assert float(off.max()) < torch.finfo(dtype).eps / 2 + (8e-5 if dtype == F16 else 5.2e-4)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("dim", [64, 128, 224])
+def test_a_maximum_that_rises_after_sums_were_put_aside(dtype, dim):
+    """Scores that rise along 40 000 slots to 64, 16-bit queries, unsplit.  Bound: scores in dim / 16 <= 14 steps of 2^-23 of 64, which enter twice, 2.2e-4; sums as in
+    test_16_bit_prompts_over_very_many_slots."""
+    need_gpu()
+    import cera_b200 as cb
+    n, heads, slots, page = 2400, 16, 40000, 32
+    g = torch.Generator("cuda").manual_seed(dim)
+    k = torch.randn(slots // page, page, 2, dim, generator=g, device="cuda")
+    k[..., 0] = torch.arange(slots, device="cuda").reshape(-1, page, 1) * (60.0 / slots)
+    k, v = k.to(dtype), (torch.rand(slots // page, page, 2, dim, generator=g, device="cuda") + 0.5).to(dtype)
+    q = torch.randn(n, heads, dim, generator=g, device="cuda") * 0.5
+    q[..., 0] = math.sqrt(dim)
+    q = q.to(dtype)
+    table = torch.randperm(slots // page, generator=torch.Generator().manual_seed(1)).to(torch.int32)[None].cuda()
+    cache = cb.PagedKv(k, v, table, _i32([slots]))
+    got = cb.paged_prefill_attention(cache, q, _i32([0, n]), 1.0 / math.sqrt(dim))
+    rows = torch.arange(0, n, 7, device="cuda")
+    kk, vv = (x[table[0].long()].reshape(slots, 2, dim).double() for x in (k, v))
+    hidden = torch.arange(slots, device="cuda") > (slots - n + rows)[:, None]
+    for h in (0, 13):
+        x = (q[rows, h].double() @ kk[:, h // 8].T / math.sqrt(dim)).masked_fill_(hidden, -math.inf)
+        want = torch.softmax(x, -1) @ vv[:, h // 8]
+        off = (got[rows, h].double() - want).abs() / want
+        assert float(off.max()) < torch.finfo(dtype).eps / 2 + (3.2e-4 if dtype == F16 else 8e-4)
