@@ -824,8 +824,8 @@ __global__ void __launch_bounds__(PD_MATH) paged_join_kernel(const PdParams p, u
         for (int v = 0; v < U; ++v) {
             const uint32_t i = i0 + v * PD_WARPS;
             const float2 s2 = i < n ? share_s[i] : make_float2(-INFINITY, 0.0f);
-            const float f = s2.x == -INFINITY ? 0.0f : pd_exp2(s2.x - m);
-            if (f == 0.0f) continue;
+            if (s2.x == -INFINITY) continue;  // a part that has met nothing is not there; one that has met a NaN is, whatever it weighs
+            const float f = pd_exp2(s2.x - m);
             l = fmaf(s2.y, f, l);
 #pragma unroll
             for (int k = 0; k < 2; ++k)

@@ -130,3 +130,33 @@ def test_a_maximum_that_rises_after_sums_were_put_aside(dtype, dim):
         want = torch.softmax(x, -1) @ vv[:, h // 8]
         off = (got[rows, h].double() - want).abs() / want
         assert float(off.max()) < torch.finfo(dtype).eps / 2 + (3.2e-4 if dtype == F16 else 8e-4)
+
+
+def _newest_slot(types, length, bad, where):
+    """The newest slot's key or value is not finite; at 33, 65 and 129 slots it has a part of the call to itself.  A NaN or infinite score makes the result NaN, one of minus infinity weighs
+    nothing; values reach their own number of the result."""
+    import cera_b200 as cb
+    c = R.Cache([length], 1, 64, 16, types[1], seed=length)
+    p, r = c.slot(0, length - 1)
+    (c.k if where == "key" else c.v)[p, r, 0, 7] = bad
+    q = _q(1, 6, 64, types[0])
+    cache = c.cuda()
+    w = torch.zeros(1, 1, c.capacity).cuda()
+    want, pv, size, js, pr = R.attend(c, 0, length - 1, q[0], 0.125)
+    fine = torch.isfinite(want)
+    want, pv = want.nan_to_num(0.0, 1.0, -1.0), torch.where(torch.isfinite(pv), pv, 0.0)
+    nan, sign = torch.isnan(R.attend(c, 0, length - 1, q[0], 0.125)[0]), torch.where(fine, 0.0, want)
+    tol = R.tolerance(want, pv, size if math.isfinite(size) else 10.0, len(js), 64, types[0], types[1])
+    for got in (cb.paged_decode_attention(cache, q.cuda(), 0.125), cb.paged_decode_attention(cache, q.cuda(), 0.125, weights=w),
+                cb.paged_prefill_attention(cache, q.cuda(), _i32([0, 1]), 0.125)):
+        got = got[0].cpu().double()
+        assert torch.equal(torch.isnan(got), nan)
+        assert torch.equal(torch.where(fine | nan, 0.0, got.nan_to_num(0.0, 1.0, -1.0)), sign)
+        R.check(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0), tol, "what is finite")
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("length", [65, 129, 33, 200])
+def test_the_newest_key_is_no_number(types, length):
+    need_gpu()
+    _newest_slot(types, length, math.nan, "key")
