@@ -204,6 +204,8 @@ struct PdMma {
         if (BF) mma_bf16(c, a, b0, b1);
         else mma_f16(c, a, b0, b1);
     }
+    // What takes the upper rows of a product with third parts: nothing but the signs (of bf16's least normal number), since zero times an infinite key or value would be a NaN.
+    static __device__ __forceinline__ uint32_t least(uint32_t hi) { return (hi & 0x80008000u) | 0x00800080u; }
     // what hi and lo leave of (x, y)
     static __device__ __forceinline__ uint32_t third(float x, float y, uint32_t hi, uint32_t lo) {
         const float2 h = unpack(hi), w = unpack(lo);
@@ -279,7 +281,7 @@ struct PdMma {
             mma(k & 1 ? sd[0] : sc[0], a, b[0], b[1]);
             mma(k & 1 ? sd[1] : sc[1], a, b[2], b[3]);
             if (THIRD) {
-                const uint32_t a3[4] = {q3[THIRD ? k : 0][0], 0u, q3[THIRD ? k : 0][1], 0u};
+                const uint32_t a3[4] = {least(qf[k][0]), q3[THIRD ? k : 0][0], least(qf[k][1]), q3[THIRD ? k : 0][1]};  // beside the lower parts
                 mma(k & 1 ? sd[0] : sc[0], a3, b[0], b[1]);
                 mma(k & 1 ? sd[1] : sc[1], a3, b[2], b[3]);
             }
@@ -290,7 +292,7 @@ struct PdMma {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float hi = sc[i >> 1][i & 1], both = hi + sc[i >> 1][(i & 1) + 2];
-            z[i] = (SPLIT && !(fabsf(both) < INFINITY) ? hi : both) * factor;  // of an infinite key the upper part says it all
+            z[i] = (SPLIT && fabsf(both) < INFINITY ? both : hi) * factor;  // of an infinite key the upper part says it all; without a lower part its rows are zeros times the key
         }
         if (mask != 0xffffu) {
 #pragma unroll
@@ -329,9 +331,9 @@ struct PdMma {
         split(w[0], w[1], wf[0], wf[1]);
         split(w[2], w[3], wf[2], wf[3]);
         if (THIRD) {
-            w3[0] = third(w[0], w[1], wf[0], wf[1]);
-            w3[2] = third(w[2], w[3], wf[2], wf[3]);
-            w3[1] = w3[3] = 0;
+            w3[1] = third(w[0], w[1], wf[0], wf[1]);
+            w3[3] = third(w[2], w[3], wf[2], wf[3]);
+            w3[0] = w3[2] = least(0);
         }
     }
     __device__ __forceinline__ void add(const PdParams &p, const uint8_t *vs, const float *) {

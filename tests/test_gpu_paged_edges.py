@@ -160,3 +160,11 @@ def _newest_slot(types, length, bad, where):
 def test_the_newest_key_is_no_number(types, length):
     need_gpu()
     _newest_slot(types, length, math.nan, "key")
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("length", [65, 129, 33, 200])
+@pytest.mark.parametrize("bad,where", [(math.inf, "key"), (-math.inf, "key"), (math.inf, "value"), (-math.inf, "value"), (math.nan, "value")])
+def test_the_newest_slot_is_infinite(types, length, bad, where):
+    need_gpu()
+    _newest_slot(types, length, bad, where)
