@@ -42,7 +42,7 @@ namespace {
 
 constexpr int PD_CTAS = 512;  // at most
 constexpr int PD_WARPS = 4, PD_MATH = 32 * PD_WARPS, PD_THREADS = PD_MATH + 64, PD_ROWS = 8;  // a warp for the keys and one for the values
-constexpr float PD_FLOOR = -3.0e38f;    // below every score that is a number
+constexpr float PD_FLOOR = -3.402823466e38f;  // no score that is a number is lower
 constexpr float PD_LIFT = 7.0f;         // weights are 2^7 at the maximum's score, 2^15 at most
 constexpr float PD_RAISE = 8.0f;
 constexpr uint32_t PD_BEGIN = 2;
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PdParams p, floa
         for (uint32_t g = 0; g < p.group; ++g) {
             const float2 ml = p.ml_unit[((size_t)(s * p.kv.hk + h) * p.chunks + g / PD_ROWS) * PD_ROWS + g % PD_ROWS];
             const float z = scores[(size_t)g * p.cap + slot];
-            if (z != -INFINITY) sum += pd_exp2(z - ml.x + PD_LIFT) / ml.y;
+            if (z != -INFINITY) sum += pd_exp2(z + (PD_LIFT - ml.x)) / ml.y;  // rounded as the sum's weights are, where scores are far from 0
         }
         weights[((size_t)s * p.kv.hk + h) * stride + slot] += sum;
     }

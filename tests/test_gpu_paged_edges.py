@@ -168,3 +168,21 @@ def test_the_newest_key_is_no_number(types, length):
 def test_the_newest_slot_is_infinite(types, length, bad, where):
     need_gpu()
     _newest_slot(types, length, bad, where)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, BF16)], ids=str)
+def test_scores_next_to_the_lowest_number(types):
+    """All scores alike at about -3.2e38 in the exponent's units: the mean of the values."""
+    need_gpu()
+    import cera_b200 as cb
+    k = torch.full((3, 64, 1, 64), 2.0 ** 60).to(types[1])
+    v = torch.randn(3, 64, 1, 64, generator=torch.Generator().manual_seed(1)).to(types[1])
+    q = torch.full((1, 2, 64), -3.2e38 / 1.4427 / 64 / 2.0 ** 60).to(types[0])
+    cache = cb.PagedKv(k.cuda(), v.cuda(), _i32([[0, 1, 2]]), _i32([150]))
+    want = v.reshape(-1, 64)[:150].double().mean(0).expand(2, 64)
+    pv = v.reshape(-1, 64)[:150].double().abs().mean(0).expand(2, 64)
+    tol = R.tolerance(want, pv, 0.0, 150, 64, types[0], types[1])
+    w = torch.zeros(1, 1, 192).cuda()
+    R.check(cb.paged_decode_attention(cache, q.cuda(), 1.0, weights=w)[0], want, tol, "decode")
+    assert float((w[0, 0, :150] * 75 - 1).abs().max()) < 1e-5 and not w[0, 0, 150:].any()
+    R.check(cb.paged_prefill_attention(cache, q.cuda(), _i32([0, 1]), 1.0)[0], want, tol, "prompt")
