@@ -325,14 +325,23 @@ __device__ __forceinline__ float pp_queries(const PpParams &p, const PpWork &w, 
     const uint32_t lane = r & 31, pieces = p.kv.dim * (uint32_t)sizeof(TQ) / 16;
     const bool live = row < w.rows;
     const uint64_t mine = live ? ((uint64_t)(w.t0 + row / p.group) * p.heads + blockIdx.y * p.group + row % p.group) * p.kv.dim : ~0ull;
-    float factor = fmaxf(fabsf(p.scale) * PAGED_LOG2E, 1.2e-38f);  // at a scale of zero all weights are alike, but for those of minus infinity
-    const bool turn = p.scale < 0.0f;
+    // a scale below zero turns the queries; one of zero is multiplied into them, so that what is not finite becomes a NaN and what is not seen stays minus infinity
+    const bool turn = p.scale < 0.0f, none = p.scale == 0.0f;
+    float factor = none ? 1.0f : fabsf(p.scale) * PAGED_LOG2E;
     if (NP == 1) {
         const uint32_t flip = turn ? 0x80008000u : 0;
+        auto zero = [](uint32_t x) {
+            const float2 f = pp_unpack<T>(x);
+            return pp_pack<T>(f.x * 0.0f, f.y * 0.0f);
+        };
         for (uint32_t c0 = 0; c0 < pieces; c0 += 4) {
             uint4 v[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) v[i] = live ? reinterpret_cast<const uint4 *>(reinterpret_cast<const TQ *>(p.q) + mine)[c0 + i] : make_uint4(0, 0, 0, 0);
+            if (none) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) v[i] = make_uint4(zero(v[i].x), zero(v[i].y), zero(v[i].z), zero(v[i].w));
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t c = c0 + i;
@@ -353,7 +362,7 @@ __device__ __forceinline__ float pp_queries(const PpParams &p, const PpWork &w, 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t rr = r - lane + i0 + u;
-            float mul = turn ? -1.0f : 1.0f;
+            float mul = none ? 0.0f : turn ? -1.0f : 1.0f;
             if (std::is_same<T, __half>::value) {
                 uint32_t most = 0;  // of absolute values, whose bits are in their order
 #pragma unroll

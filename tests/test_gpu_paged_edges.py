@@ -186,3 +186,53 @@ def test_scores_next_to_the_lowest_number(types):
     R.check(cb.paged_decode_attention(cache, q.cuda(), 1.0, weights=w)[0], want, tol, "decode")
     assert float((w[0, 0, :150] * 75 - 1).abs().max()) < 1e-5 and not w[0, 0, 150:].any()
     R.check(cb.paged_prefill_attention(cache, q.cuda(), _i32([0, 1]), 1.0)[0], want, tol, "prompt")
+
+
+# ---- scales ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.125, 1e-39, -1e-39])
+def test_scales(types, scale):
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([200], 2, 64, 16, types[1], seed=3)
+    q = _q(30, 4, 64, types[0])
+    got = cb.paged_prefill_attention(c.cuda(), q.cuda(), _i32([0, 30]), scale, window=50, n_sink=3)
+    one = cb.paged_decode_attention(c.cuda(), q[29:].cuda(), scale, window=50, n_sink=3)
+    for i in range(30):
+        want, pv, size, js, _ = R.attend(c, 0, 170 + i, q[i], scale, 50, 3)
+        tol = R.tolerance(want, pv, size, len(js), 64, types[0], types[1])
+        R.check(got[i], want, tol, f"query {i}")
+        if i == 29:
+            R.check(one[0], want, tol, "decode")
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_a_scale_that_is_no_number(types):
+    """Every row that sees a slot is NaN; one that sees none is zero."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([20], 2, 64, 16, types[1], seed=3)
+    q = _q(25, 4, 64, types[0]).cuda()
+    got = cb.paged_prefill_attention(c.cuda(), q, _i32([0, 25]), math.nan)
+    assert not got[:5].any() and torch.isnan(got[5:]).all()
+    assert torch.isnan(cb.paged_decode_attention(c.cuda(), q[:1], math.nan)).all()
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("in_query", [False, True])
+def test_a_scale_of_zero_times_what_is_not_finite(types, bad, in_query):
+    """Zero times infinity is NaN, for those who see it."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([90], 1, 64, 16, types[1], seed=3)
+    q = _q(90, 2, 64, types[0])
+    if in_query:
+        q[60:, :, 5] = bad
+    else:
+        p, r = c.slot(0, 60)
+        c.k[p, r, 0, 5] = bad
+    got = cb.paged_prefill_attention(c.cuda(), q.cuda(), _i32([0, 90]), 0.0)
+    assert torch.isfinite(got[:60]).all() and torch.isnan(got[60:]).all()
+    assert torch.isnan(cb.paged_decode_attention(c.cuda(), q[89:].cuda(), 0.0)).all()
