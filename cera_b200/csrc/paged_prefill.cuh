@@ -168,8 +168,10 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams 
             out[128 * k + 4 * lane + i] = from_f32<TQ>(sees ? y[i] : 0.0f);
         }
     }
-    if (__any_sync(0xffffffffu, check != 0.0f))
+    if (__any_sync(0xffffffffu, check != 0.0f)) {
+        __syncwarp();  // other lanes stored these numbers
         paged_attend_row<T, TQ>(p.kv, p.mask, s, h / p.group, len - behind, reinterpret_cast<const TQ *>(p.q) + r * p.kv.dim, p.scale, out);
+    }
 }
 
 // CTAs along the rows (an upper bound: the portions' lengths are on the device) and the splits of the keys.
