@@ -97,6 +97,14 @@ int32_t check_heads(const char *what, const PagedView &v, int32_t type, int32_t 
     return CERA_CUDA_OK;
 }
 
+// A result goes where its queries are, or apart from them.
+int32_t check_out(const char *what, const void *q, const void *out, int32_t q_type, const PagedView &v, size_t n, size_t n_heads) {
+    const uintptr_t a = (uintptr_t)q, b = (uintptr_t)out;
+    if (!q || !out || ((a | b) & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: queries or result null or off a 16-byte boundary", what);
+    if (a != b && (a < b ? b - a : a - b) < n * n_heads * v.dim * elem(q_type)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: the result covers a part of the queries", what);
+    return CERA_CUDA_OK;
+}
+
 // Rows (token, head of a KV head) are counted in 31 bits.
 int32_t check_tokens(const char *what, const PagedView &v, size_t n_heads, size_t n_tokens) {
     if (n_tokens > 0x7fffffffu / (n_heads / v.hk)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: %zu tokens", what, n_tokens);
@@ -191,7 +199,7 @@ int32_t cera_cuda_paged_decode_attention(const cera_cuda_paged_kv *kv, const voi
     if (weights_dev && weights_stride < (size_t)v.max_pages * v.page_size)
         return fail(CERA_CUDA_ERR_BAD_ARG, "%s: weights of %zu slots (%zu)", what, weights_stride, (size_t)v.max_pages * v.page_size);
     if (v.n_seqs == 0) return CERA_CUDA_OK;
-    if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: queries or result null or off a 16-byte boundary", what);
+    CERA_TRY(check_out(what, q_dev, out_dev, q_type, v, v.n_seqs, n_heads));
     CERA_TRY(check_workspace(what, workspace_dev, workspace_bytes, paged_decode_workspace(v, n_heads, weights_dev != nullptr)));
     return launch_paged_decode(v, kv->type, q_dev, q_type, n_heads, scale, PagedMask{window, n_sink}, weights_dev, weights_stride, out_dev, workspace_dev,
                                (cudaStream_t)stream);
@@ -216,7 +224,7 @@ int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const vo
     CERA_TRY(check_tokens(what, v, n_heads, n_tokens));
     if (n_tokens == 0 || v.n_seqs == 0) return CERA_CUDA_OK;
     if (!starts_dev) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: no starts", what);
-    if (!q_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15)) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: queries or result null or off a 16-byte boundary", what);
+    CERA_TRY(check_out(what, q_dev, out_dev, q_type, v, n_tokens, n_heads));
     CERA_TRY(check_workspace(what, workspace_dev, workspace_bytes, paged_prefill_workspace(v, kv->type, n_heads, n_tokens)));
     return launch_paged_prefill(v, kv->type, q_dev, q_type, n_heads, starts_dev, n_tokens, scale, PagedMask{window, n_sink}, out_dev, workspace_dev,
                                 (cudaStream_t)stream);

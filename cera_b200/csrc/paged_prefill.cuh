@@ -160,17 +160,20 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams 
     float check = l > 0.0f || !sees ? 0.0f : NAN;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        if (128 * k + 4 * lane >= p.kv.dim) continue;
-        const float y[4] = {o[k].x / l, o[k].y / l, o[k].z / l, o[k].w / l};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (sees) check = fmaf(y[i], 0.0f, check);
-            out[128 * k + 4 * lane + i] = from_f32<TQ>(sees ? y[i] : 0.0f);
-        }
+        o[k] = make_float4(o[k].x / l, o[k].y / l, o[k].z / l, o[k].w / l);
+        if (sees && 128 * k + 4 * lane < p.kv.dim) check = fmaf(o[k].x, 0.0f, fmaf(o[k].y, 0.0f, fmaf(o[k].z, 0.0f, fmaf(o[k].w, 0.0f, check))));
     }
-    if (__any_sync(0xffffffffu, check != 0.0f)) {
-        __syncwarp();  // other lanes stored these numbers
+    if (__any_sync(0xffffffffu, check != 0.0f)) {  // nothing is stored yet: the queries may be where the result goes
+        __syncwarp();
         paged_attend_row<T, TQ>(p.kv, p.mask, s, h / p.group, len - behind, reinterpret_cast<const TQ *>(p.q) + r * p.kv.dim, p.scale, out);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (128 * k + 4 * lane >= p.kv.dim) continue;
+        const float y[4] = {o[k].x, o[k].y, o[k].z, o[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[128 * k + 4 * lane + i] = from_f32<TQ>(sees ? y[i] : 0.0f);
     }
 }
 

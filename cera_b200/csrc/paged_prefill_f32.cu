@@ -208,11 +208,16 @@ __global__ void __launch_bounds__(PF_THREADS) paged_prefill_f32_kernel(const PpP
 #pragma unroll
         for (int i = 0; i < C::NV; ++i) {
             if (!live || (g16 + 16 * i) * 4 >= dim) continue;
-            const float4 o = make_float4(acc[r][i].x * f, acc[r][i].y * f, acc[r][i].z * f, acc[r][i].w * f);
+            const float4 o = acc[r][i] = make_float4(acc[r][i].x * f, acc[r][i].y * f, acc[r][i].z * f, acc[r][i].w * f);
             check = fmaf(o.x, 0.0f, fmaf(o.y, 0.0f, fmaf(o.z, 0.0f, fmaf(o.w, 0.0f, check))));
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out) + place * dim + (g16 + 16 * i) * 4) = pos[r] >= 0 ? o : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         const uint32_t bad = __ballot_sync(0xffffffffu, pos[r] >= 0 && check != 0.0f);
+        if (!(bad >> (lane & 16) & 0xffffu)) {  // what is computed again is stored then: the queries may be where the result goes
+#pragma unroll
+            for (int i = 0; i < C::NV; ++i)
+                if (live && (g16 + 16 * i) * 4 < dim)
+                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out) + place * dim + (g16 + 16 * i) * 4) = pos[r] >= 0 ? acc[r][i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
         again |= (bad & 0xffffu ? 1u << r : 0) | (bad >> 16 ? 1u << (PF_EACH + r) : 0);
     }
     for (; again; again &= again - 1) {

@@ -637,7 +637,15 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
     TQ *out = reinterpret_cast<TQ *>(p.out) + place * p.kv.dim;
     const float f = 1.0f / l;
     float check = l > 0.0f && m != PP_FLOOR ? 0.0f : NAN;
-    for (uint32_t d = 0; d < p.kv.dim; d += 32) {
+    for (uint32_t d = 0; done && d < p.kv.dim; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(to + d, o);
+        tmem_wait_ld32(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) check = fmaf(__uint_as_float(o[e]) * f, 0.0f, check);
+    }
+    uint32_t again = __ballot_sync(0xffffffffu, pos >= 0 && check != 0.0f);
+    for (uint32_t d = 0; d < p.kv.dim; d += 32) {  // what is computed again is stored then: the queries may be where the result goes
         uint32_t o[32];
         if (done) {
             tmem_ld32(to + d, o);
@@ -649,13 +657,11 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
 #pragma unroll
             for (uint32_t k = 0; k < 16 / sizeof(TQ); ++k) {
                 const float x = done ? __uint_as_float(o[e + k]) * f : 0.0f;
-                check = fmaf(x, 0.0f, check);
                 y[k] = from_f32<TQ>(pos >= 0 ? x : 0.0f);
             }
-            if (live) *reinterpret_cast<uint4 *>(out + d + e) = *reinterpret_cast<const uint4 *>(y);
+            if (live && !(again >> lane & 1)) *reinterpret_cast<uint4 *>(out + d + e) = *reinterpret_cast<const uint4 *>(y);
         }
     }
-    uint32_t again = __ballot_sync(0xffffffffu, pos >= 0 && check != 0.0f);
     for (; again; again &= again - 1) {
         const uint32_t rr = a + quad * 32 + __ffs(again) - 1;
         const size_t pl = ((size_t)(w.t0 + rr / p.group) * p.heads + blockIdx.y * p.group + rr % p.group) * p.kv.dim;

@@ -146,7 +146,7 @@ def paged_decode_attention(cache, q, scale, window=0, n_sink=0, weights=None, ou
     """Attention of every sequence's newest token, which is in its last slot: q [n_seqs, n_heads, head_dim] of the cache's type or float32;
     the result is of q's type.  window: only that many last slots are seen, and the first n_sink (0: all).  weights, float32
     [n_seqs, n_kv_heads, at least capacity], has the probabilities of a KV head's query heads added to their slots.  A sequence
-    without slots gives zeros.  Calls that may overlap need a workspace each; by default every call has its own."""
+    without slots gives zeros.  `out` may be q.  Calls that may overlap need a workspace each; by default every call has its own."""
     stream, ref = cache._stream(), cache._ref
     qp = cache._rows(q, "q", cache.n_seqs, None)
     _visible(window, n_sink)
@@ -165,7 +165,7 @@ def paged_decode_attention(cache, q, scale, window=0, n_sink=0, weights=None, ou
 def paged_prefill_attention(cache, q, starts, scale, window=0, n_sink=0, out=None, workspace=None):
     """Causal attention of portions of prompts: q [n_tokens, n_heads, head_dim], of which sequence s has [starts[s], starts[s + 1])
     (int32 [n_seqs + 1], ascending from 0) in its last slots.  Types, window and n_sink as in paged_decode_attention, the window counted
-    back from each query.  Rows past starts[n_seqs] are left as they are in `out`, and undefined without one."""
+    back from each query; `out` may be q.  Rows past starts[n_seqs] are left as they are in `out`, and undefined without one."""
     stream, ref = cache._stream(), cache._ref
     qp, sp = cache._rows(q, "q", None, None), cache._starts(starts)
     _visible(window, n_sink)

@@ -240,7 +240,8 @@ CERA_API int32_t cera_cuda_paged_append(const cera_cuda_paged_kv *kv, const void
                                         void *stream);
 /* Attention of the newest token of every sequence, in slot p = seq_lens[s] - 1: q_dev and out_dev are
  * [n_seqs][n_heads][head_dim] of q_type, the cache's type or F32; n_heads a multiple of n_kv_heads.  Slots j <= p are seen;
- * with window != 0 those with j < n_sink or j > p - window.  A row that sees nothing is 0.  weights_dev (optional,
+ * with window != 0 those with j < n_sink or j > p - window.  A row that sees nothing is 0.  out_dev may be q_dev; a part of it
+ * it may not be.  weights_dev (optional,
  * [n_seqs][n_kv_heads][weights_stride]): the probabilities of a KV head's query heads are added to their slots.  workspace_dev
  * holds cera_cuda_paged_decode_attention_workspace_bytes(...) bytes (0: an argument is refused) on a 16-byte boundary; calls that may overlap need one each. */
 CERA_API size_t cera_cuda_paged_decode_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads,
@@ -250,7 +251,7 @@ CERA_API int32_t cera_cuda_paged_decode_attention(const cera_cuda_paged_kv *kv, 
                                                   float *weights_dev, size_t weights_stride, void *out_dev,
                                                   void *workspace_dev, size_t workspace_bytes, void *stream);
 /* Causal attention of the newest tokens of every sequence, [starts[s], starts[s + 1]) of q_dev [n_tokens][n_heads][head_dim]
- * in its last slots, with the same window and types.  Rows of out_dev past starts[n_seqs] stay as they are. */
+ * in its last slots, with the same window and types; out_dev may be q_dev here too.  Rows of out_dev past starts[n_seqs] stay as they are. */
 CERA_API size_t cera_cuda_paged_prefill_attention_workspace_bytes(const cera_cuda_paged_kv *kv, size_t n_heads,
                                                                  size_t n_tokens);
 CERA_API int32_t cera_cuda_paged_prefill_attention(const cera_cuda_paged_kv *kv, const void *q_dev, int32_t q_type,

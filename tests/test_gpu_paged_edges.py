@@ -236,3 +236,26 @@ def test_a_scale_of_zero_times_what_is_not_finite(types, bad, in_query):
     got = cb.paged_prefill_attention(c.cuda(), q.cuda(), _i32([0, 90]), 0.0)
     assert torch.isfinite(got[:60]).all() and torch.isnan(got[60:]).all()
     assert torch.isnan(cb.paged_decode_attention(c.cuda(), q[89:].cuda(), 0.0)).all()
+
+
+# ---- a result over its queries --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("new,length", [(90, 200), (3, 1000), (300, 400)])
+def test_a_result_may_go_where_its_queries_are(types, new, length):
+    """With an infinite value that some rows do not see: those are computed a second time, from the queries."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([length], 2, 64, 16, types[1], seed=3)
+    p, r = c.slot(0, length - new // 2 - 1)
+    c.v[p, r, 0, 5] = math.inf
+    q = _q(new, 4, 64, types[0]).cuda()
+    starts = _i32([0, new])
+    want = cb.paged_prefill_attention(c.cuda(), q, starts, 0.125)
+    over = q.clone()
+    assert cb.paged_prefill_attention(c.cuda(), over, starts, 0.125, out=over) is over
+    assert torch.equal(over.isnan(), want.isnan()) and torch.equal(over.nan_to_num(0.0), want.nan_to_num(0.0))
+    want = cb.paged_decode_attention(c.cuda(), q[:1], 0.125)
+    over = q[:1].clone()
+    cb.paged_decode_attention(c.cuda(), over, 0.125, out=over)
+    assert torch.equal(over.isnan(), want.isnan()) and torch.equal(over.nan_to_num(0.0), want.nan_to_num(0.0))
