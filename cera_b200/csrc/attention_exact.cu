@@ -771,7 +771,7 @@ int32_t launch_decode_attention_exact(const float *q, const void *kc, const void
 static const bool g_ax_status_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_ax_status, sizeof(v));
-    return (uint32_t)v << 23;  // bits 23, 24
+    return STATUS_ATTENTION_EXACT.of(v);
 });
 
 }  // namespace cera

@@ -19,7 +19,7 @@ __device__ unsigned int g_attention_tc_status = 0;
 static const bool g_attention_tc_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_attention_tc_status, sizeof(v));
-    return (uint32_t)v << 20;
+    return STATUS_ATTENTION_TC.of(v);
 });
 
 namespace {

@@ -17,6 +17,25 @@ int32_t check_cuda(cudaError_t e, const char *what);
 // Kernels with bounded waits keep a status word in device memory; the file that owns one registers its reader here
 // (at load time) and cera_cuda_kernel_status ORs them all.
 bool register_kernel_status(uint32_t (*reader)());
+// Whose bits of that word are whose: a kernel's own word, one bit a role that gave up, shifted to the first of its bits.
+struct StatusBits {
+    uint32_t first, count;
+    constexpr uint32_t mask() const { return ((1u << count) - 1) << first; }
+    uint32_t of(uint32_t word) const { return (word << first) & mask(); }
+};
+constexpr StatusBits STATUS_GEMV_TMA = {0, 2}, STATUS_PAGED_DECODE = {2, 2}, STATUS_PAGED_PREFILL = {4, 3}, STATUS_GEMM_TC = {8, 5}, STATUS_GEMV_EXACT = {13, 2}, STATUS_DENSE_GEMM_TC = {17, 3},
+                     STATUS_ATTENTION_TC = {20, 3}, STATUS_ATTENTION_EXACT = {23, 2}, STATUS_GEMM_TCQ = {25, 4};
+constexpr bool status_bits_apart() {
+    constexpr StatusBits all[] = {STATUS_GEMV_TMA, STATUS_PAGED_DECODE, STATUS_PAGED_PREFILL, STATUS_GEMM_TC, STATUS_GEMV_EXACT, STATUS_DENSE_GEMM_TC, STATUS_ATTENTION_TC, STATUS_ATTENTION_EXACT,
+                                  STATUS_GEMM_TCQ};
+    uint32_t taken = 0;
+    for (const StatusBits &b : all) {
+        if (b.first + b.count > 32 || (taken & b.mask())) return false;
+        taken |= b.mask();
+    }
+    return true;
+}
+static_assert(status_bits_apart(), "two kernels report in one bit");
 void count_launch(int n = 1);      // bumps the library-wide kernel launch counter
 uint64_t launches_so_far();
 

@@ -22,7 +22,7 @@ __device__ unsigned int g_dense_tc_status = 0;
 static const bool g_dense_tc_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_dense_tc_status, sizeof(v));
-    return (uint32_t)v << 17;
+    return STATUS_DENSE_GEMM_TC.of(v);
 });
 
 namespace {

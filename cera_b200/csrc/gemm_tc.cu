@@ -1215,7 +1215,7 @@ int32_t weight_prepare_tc(cera_cuda_weight *w, bool *built) {
 static const bool g_tc_status_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(v));
-    return (uint32_t)v << 8;
+    return STATUS_GEMM_TC.of(v);
 });
 
 size_t gemm_parts_bytes() { return (size_t)TC_SHARES * sm_count() * (2 * TC_BN * TC_BM * 4); }

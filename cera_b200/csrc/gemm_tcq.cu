@@ -739,7 +739,7 @@ int32_t launch_gemm_tcq_grouped(const WeightView *ws, float *const *outs, int n_
 static const bool g_tcq_status_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_tcq_status, sizeof(v));
-    return (uint32_t)v << 25;
+    return STATUS_GEMM_TCQ.of(v);
 });
 
 }  // namespace cera

@@ -671,7 +671,7 @@ int32_t launch_exact_typed(const ExactParams &p0, cudaStream_t st) {
 static const bool g_xg_status_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_xg_status, sizeof(v));
-    return (uint32_t)v << 16;
+    return STATUS_GEMV_EXACT.of(v);
 });
 
 // CERA_CUDA_GEMV=rows keeps the decode GEMVs on the register-streaming kernel whose f32 order is its own (A/B runs); read once.

@@ -334,11 +334,11 @@ int32_t launch_gemv_tma(const GemvSeg *segs, int n_segs, const ActView &x, int e
     return CERA_CUDA_OK;
 }
 
-// low bits: roles of the TMA-staged GEMV
+// roles of the TMA-staged GEMV
 static const bool g_tma_status_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_tma_status, sizeof(v));
-    return (uint32_t)v;
+    return STATUS_GEMV_TMA.of(v);
 });
 
 }  // namespace cera

@@ -35,7 +35,7 @@ __device__ unsigned int g_paged_decode_status = 0;
 static const bool g_paged_decode_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_paged_decode_status, sizeof(v));
-    return (uint32_t)v << 24;
+    return STATUS_PAGED_DECODE.of(v);
 });
 
 namespace {

@@ -31,7 +31,7 @@ __device__ unsigned int g_paged_prefill_status = 0;
 static const bool g_paged_prefill_registered = register_kernel_status([] {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_paged_prefill_status, sizeof(v));
-    return (uint32_t)v << 26;
+    return STATUS_PAGED_PREFILL.of(v);
 });
 
 namespace {

@@ -21,3 +21,22 @@ def test_a_row_that_is_computed_again_is_stored_behind_what_was_stored_first():
             ahead = text[:call.start()].rstrip()
             assert "__syncwarp();" in ahead[-400:] and ahead.rindex("__syncwarp();") > max(ahead.rfind("__any_sync("), ahead.rfind("__ballot_sync(")), name
     assert seen == 3
+
+
+def test_every_kernel_reports_in_bits_of_its_own():
+    """The compiler checks that the bits lie apart; here: every reader takes its own, and no role of a kernel is outside of them."""
+    table = {n: (int(a), int(c)) for n, a, c in re.findall(r"(STATUS_\w+) = \{(\d+), (\d+)\}", _text("common.cuh"))}
+    bits = [b for a, c in table.values() for b in range(a, a + c)]
+    assert len(set(bits)) == len(bits) and max(bits) < 32
+    assert all(re.search(r"all\[\] = \{[^}]*\b%s\b" % n, _text("common.cuh")) for n in table)
+    used = {}
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith(".cu") or name == "runtime.cu" or "register_kernel_status(" not in _text(name):
+            continue
+        text = _text(name)
+        owner, = re.findall(r"return (STATUS_\w+)\.of\(v\);", text)
+        roles = [int(r) for call in re.findall(r"\b(?:mbar_wait\w*|arrived)\(([^;{]*)", text) for r in re.findall(r", (\d+)u\)", call)]
+        assert roles and max(roles) < 1 << table[owner][1], (name, roles)
+        assert all(r & (r - 1) == 0 for r in roles), (name, roles)
+        used[owner] = name
+    assert set(used) == set(table)
