@@ -901,7 +901,7 @@ int32_t pd_launch(PdParams &p, int type, float *weights, size_t weights_stride, 
     CERA_CUDA_TRY(launch_k(kernel, dim3(G), dim3(PD_THREADS), smem, st, mk, mv, p));
     CERA_CUDA_TRY(launch_k(paged_join_kernel<TQ, W::TILE>, dim3(p.kv.n_seqs * p.kv.hk * p.chunks, std::min<uint32_t>(p.group, PD_ROWS)), dim3(PD_MATH), 0, st, p, G));
     if (!weights) return CERA_CUDA_OK;
-    const uint32_t wide = (uint32_t)std::min<size_t>((p.cap + 255) / 256, std::max<size_t>(1, 148 * 8 / std::max(1u, p.kv.n_seqs * p.kv.hk)));
+    const uint32_t wide = (uint32_t)std::min<size_t>((p.cap + 255) / 256, std::max<size_t>(1, 8 * (size_t)sm_count() / std::max(1u, p.kv.n_seqs * p.kv.hk)));
     return check_cuda(launch_k(paged_weigh_kernel, dim3(std::max(1u, wide), p.kv.hk, p.kv.n_seqs), dim3(256), 0, st, p, weights, weights_stride), "paged decode weights launch");
 }
 

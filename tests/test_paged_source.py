@@ -40,3 +40,9 @@ def test_every_kernel_reports_in_bits_of_its_own():
         assert all(r & (r - 1) == 0 for r in roles), (name, roles)
         used[owner] = name
     assert set(used) == set(table)
+
+
+def test_no_number_of_sms_by_hand():
+    for name in sorted(os.listdir(CSRC)):
+        if name.startswith("paged"):
+            assert not re.search(r"\b148\b", _text(name)), name
