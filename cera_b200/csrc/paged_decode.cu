@@ -602,7 +602,13 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
         };
         find();
         const uint32_t me = elect_one();
-        for (uint32_t x = 0; at.behind(end); ++x) {
+        // shared memory must outlive the copies in flight, those of the stages before tile n: whoever reads them may give up while they are
+        auto drain = [&](uint32_t n) {
+            for (uint32_t y = n > ST ? n - ST : 0; y < n; ++y)
+                for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % ST], y / ST & 1); ++i) __nanosleep(40);
+        };
+        uint32_t x = 0;
+        for (; at.behind(end); ++x) {
             const uint32_t st = x % ST;
             const uint32_t slot0 = at.slot(at.tile, TILE), h = at.unit / p.chunks;
             uint32_t mask[2];
@@ -616,11 +622,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
             }
             at.step(line, p.kv, p.mask);
             if (at.behind(end)) find();  // its answer is not needed before the next tile
-            if (!tma::mbar_wait_warp(&empty_s[st], (x / ST & 1) ^ 1, &abort_s, status, 1u)) {  // given up: shared memory must outlive the copies in flight
-                for (uint32_t y = x > ST ? x - ST : 0; y < x; ++y)
-                    for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % ST], y / ST & 1); ++i) __nanosleep(40);
-                return;
-            }
+            if (!tma::mbar_wait_warp(&empty_s[st], (x / ST & 1) ^ 1, &abort_s, status, 1u)) return drain(x);
             if (!is_v && lane < 2) mask_s[st][lane] = lane ? mask[1] : mask[0];
             __syncwarp();
             uint8_t *to = half + st * S::STAGE;
@@ -647,6 +649,7 @@ __global__ void __launch_bounds__(PD_THREADS, DP <= 128 ? 2 : 1) paged_decode_ke
                 if (lane == 0) tma::mbar_arrive(&full[st]);  // the mask's
             }
         }
+        drain(x);
         return;
     }
 

@@ -162,7 +162,7 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
         }
     };
     uint32_t parts = 0;
-    // given up: shared memory must outlive the copies in flight, those of the stages before tile n and, if the last was not whole, its own
+    // shared memory must outlive the copies in flight, those of the stages before tile n and, if the last was not whole, its own: whoever reads them may give up while they are
     auto drain = [&](uint32_t n, bool all) {
         for (uint32_t y = n > C::ST ? n - C::ST : 0; y < n; ++y)
             for (uint32_t i = 0; i < tma::SPIN_LIMIT && !tma::mbar_test(&full[y % C::ST], y / C::ST & 1); ++i) __nanosleep(40);
@@ -237,6 +237,7 @@ __device__ __forceinline__ void pp_load(const PpParams &p, const PpWork &w, cons
             if (lane == 0) tma::mbar_arrive(&full[st]);
         }
     }
+    drain(w.x1 - w.x0, true);
 }
 
 // The products, a warp that stays together (descriptors live in registers that a warp has once: a branch of one lane around them mixes them up): of each tile of rows

@@ -46,3 +46,17 @@ def test_no_number_of_sms_by_hand():
     for name in sorted(os.listdir(CSRC)):
         if name.startswith("paged"):
             assert not re.search(r"\b148\b", _text(name)), name
+
+
+def test_loaders_wait_for_their_copies_before_they_leave():
+    """Shared memory may not go to another CTA with a copy on its way into it: where a loader gives a wait up, and at its end too, since those who read what it loaded may give up later."""
+    decode = _text("paged_decode.cu")
+    decode = decode[decode.index("if (warp >= PD_WARPS) {"):decode.index("float *qs = values")]
+    prompt = _text("paged_prefill_tc.cu")
+    prompt = prompt[prompt.index("void pp_load("):prompt.index("void pp_multiply(")]
+    for text, waits in ((decode, 1), (prompt, 2)):
+        body = text[:text.rindex("drain(")]
+        assert re.search(r"auto drain = .*?SPIN_LIMIT.*?mbar_test\(&full\[", text, re.S)
+        given_up = re.findall(r"if \(!tma::mbar_wait_warp\([^;]*?status, \d+u\)\) return drain\(", body)
+        assert len(given_up) == waits == len(re.findall(r"mbar_wait_warp\(", text))
+        assert re.fullmatch(r"drain\([^;]*\);\s*(return;\s*)?\}\s*(template <[^{]*)?", text[text.rindex("drain("):]), text[text.rindex("drain("):]
