@@ -259,3 +259,63 @@ def test_a_result_may_go_where_its_queries_are(types, new, length):
     over = q[:1].clone()
     cb.paged_decode_attention(c.cuda(), over, 0.125, out=over)
     assert torch.equal(over.isnan(), want.isnan()) and torch.equal(over.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+# ---- forms that only some calls reach -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("heads,hk,dim", [(8, 1, 64), (5, 1, 128), (24, 2, 64), (17, 1, 96), (20, 1, 160), (6, 1, 256)])
+def test_weights_of_large_groups(types, heads, hk, dim):
+    """Five to eight heads a KV head, more than eight, and wide heads."""
+    need_gpu()
+    import cera_b200 as cb
+    for window, sink in ((0, 0), (90, 4)):
+        _decode_case(cb, R.Cache([1, 300, 0, 64, 130], hk, dim, 16, types[1], seed=heads), heads, types[0], window, sink, weights=True)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("longest,budget", [(9000, 900), (9000, 8500), (20000, 3000), (20000, 19500)])
+def test_clusters_evict_several_sequences(longest, budget, in_place):
+    """Clusters of four and eight CTAs a pair, ragged lengths, some within the budget; rows moved by a second launch and by the first."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([0, 0, 0, 0], 2, 32, 64, F16)
+    c.lens, c.wide = [longest, 5, 0, longest - 400], -(-longest // 64)
+    c.pages, c.capacity = 4 * c.wide, c.wide * 64
+    c.table = torch.randperm(c.pages, generator=torch.Generator().manual_seed(1)).to(torch.int32).reshape(4, c.wide)
+    c.k, c.v = (torch.randn(c.pages, 64, 2, 32, generator=torch.Generator().manual_seed(i)).half() for i in (2, 3))
+    _evict_case(cb, c, *_track(c, 5, ties=True), budget, 4, 30, in_place)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_a_workspace_of_ones_own(types):
+    """Filled with NaN, used by one call after the other, of the size that is asked for and not a byte less."""
+    need_gpu()
+    import ctypes as C
+    import cera_b200 as cb
+    from cera_b200._lib import lib
+    c = R.Cache([3000, 70, 0], 2, 64, 16, types[1], seed=80)
+    cache = c.cuda()
+    q, starts = _q(9, 8, 64, types[0]).cuda(), _i32([0, 4, 9, 9])
+    w = [torch.zeros(3, 2, c.capacity).cuda() for _ in range(2)]
+    ref = C.byref(cache._desc)
+    calls = [(lambda **kw: cb.paged_decode_attention(cache, q[:3].contiguous(), 0.125, **kw), lib.cera_cuda_paged_decode_attention_workspace_bytes(ref, 8, 0)),
+             (lambda **kw: cb.paged_decode_attention(cache, q[:3].contiguous(), 0.125, weights=w["workspace" in kw], **kw),
+              lib.cera_cuda_paged_decode_attention_workspace_bytes(ref, 8, 1)),
+             (lambda **kw: cb.paged_prefill_attention(cache, q, starts, 0.125, **kw), lib.cera_cuda_paged_prefill_attention_workspace_bytes(ref, 8, 9))]
+    ws = torch.full((max(n for _, n in calls) + 64,), 255, dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        for call, need in calls:
+            want = call()
+            out = torch.full_like(want, 9.0)
+            assert call(workspace=ws[:need], out=out) is out and torch.equal(out, want)
+            with pytest.raises(ValueError, match="workspace"):
+                call(workspace=ws[:need - 1])
+    assert torch.equal(w[0], w[1])
+
+
+def test_no_wait_of_these_kernels_ran_out():
+    need_gpu()
+    from cera_b200._lib import kernel_status
+    torch.cuda.synchronize()
+    assert kernel_status() == 0
