@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView kv, c
     const uint32_t t = blockIdx.x, s = paged_seq_of(starts, kv.n_seqs, t);
     if (s >= kv.n_seqs) return;
     const uint32_t len = paged_len(kv, s), behind = starts ? (uint32_t)starts[s + 1] - t : 1;  // this token and those behind it in its sequence
-    if (behind > len) return;
+    if (behind - 1 >= len) return;  // also where starts do not ascend
     const uint32_t slot = len - behind;
     for (uint32_t h = threadIdx.x; h < kv.hk; h += blockDim.x) {
         const size_t at = ((size_t)s * kv.hk + h) * track_stride + slot;

@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PpParams 
     }
     if (s >= p.kv.n_seqs) return;
     TQ *out = reinterpret_cast<TQ *>(p.out) + r * p.kv.dim;
-    const uint32_t len = paged_len(p.kv, s), behind = (uint32_t)p.starts[s + 1] - t;
-    const bool sees = behind <= len;
+    const uint32_t len = paged_len(p.kv, s), behind = (uint32_t)min(p.starts[s + 1], (int32_t)p.n) - t;
+    const bool sees = behind - 1 < len;  // (starts that do not ascend see nothing)
     float check = l > 0.0f || !sees ? 0.0f : NAN;
 #pragma unroll
     for (int k = 0; k < K; ++k) {

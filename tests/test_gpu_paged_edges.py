@@ -319,3 +319,27 @@ def test_no_wait_of_these_kernels_ran_out():
     from cera_b200._lib import kernel_status
     torch.cuda.synchronize()
     assert kernel_status() == 0
+
+
+@pytest.mark.parametrize("starts", [[0, 9, 2, 2], [0, 2, 9, 1], [0, 12, 12, 12], [5, 5, 5, 12], [0, -4, 3, 3], [3, 2, 1, 0]])
+def test_starts_that_do_not_ascend_touch_nothing_else(starts):
+    """They are not allowed, and what they give is not said; what lies beside the sequences' slots stays as it was."""
+    need_gpu()
+    import cera_b200 as cb
+    c = R.Cache([48, 48, 48], 2, 64, 16, F16, seed=7, spare=0)
+    cache = c.cuda()
+    spare = next(p for p in range(c.pages) if p not in set(c.table.flatten().tolist()))
+    table = torch.full((5, 3), spare, dtype=torch.int32)  # a slot past the capacity would find the page that no sequence has
+    table[1:4] = c.table
+    whole = table.cuda()
+    cache = cb.PagedKv(cache.k_pages, cache.v_pages, whole[1:4], cache.seq_lens)
+    k = torch.ones(9, 2, 64, dtype=F16, device="cuda")
+    w, p = torch.full((5, 2, 48), 3.0).cuda(), torch.full((5, 2, 48), 3, dtype=torch.int32).cuda()
+    cb.paged_append(cache, k, k, _i32(starts), weights=w[1:4], positions=p[1:4])
+    for x in (w, p):
+        assert (x[0] == 3).all() and (x[4] == 3).all()
+    assert torch.isnan(c.kd[spare]).all() and torch.isnan(c.vd[spare]).all()
+    q = torch.full((11, 4, 64), 5.0, dtype=F16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    cb.paged_prefill_attention(cache, q[:9], _i32(starts), 0.125, out=out[:9])
+    assert (out[9:] == 7.0).all() and (whole[0] == spare).all() and (whole[4] == spare).all()
