@@ -343,3 +343,42 @@ def test_starts_that_do_not_ascend_touch_nothing_else(starts):
     out = torch.full_like(q, 7.0)
     cb.paged_prefill_attention(cache, q[:9], _i32(starts), 0.125, out=out[:9])
     assert (out[9:] == 7.0).all() and (whole[0] == spare).all() and (whole[4] == spare).all()
+
+
+def test_as_many_sequences_as_there_may_be():
+    need_gpu()
+    import cera_b200 as cb
+    lens = [(7 * i) % 5 + (200 if i % 1000 == 999 else 0) for i in range(4096)]
+    c = R.Cache([0], 2, 32, 8, F16)
+    c.lens, c.wide = lens, 26
+    c.pages, c.capacity = sum(-(-x // 8) for x in lens), 26 * 8
+    c.table, at = torch.full((4096, 26), -1, dtype=torch.int32), 0
+    for s, x in enumerate(lens):
+        n = -(-x // 8)
+        c.table[s, :n] = torch.arange(at, at + n)
+        at += n
+    c.k, c.v = (torch.randn(c.pages, 8, 2, 32, generator=torch.Generator().manual_seed(i)).half() for i in (2, 3))
+    cache = c.cuda()
+    q = _q(4096, 4, 32, F16)
+    w = torch.zeros(4096, 2, 208).cuda()
+    got = cb.paged_decode_attention(cache, q.cuda(), 0.2, weights=w).cpu()
+    last = [i for i, x in enumerate(lens) if x]
+    starts = torch.zeros(4097, dtype=torch.int32)
+    starts[1:] = torch.tensor([int(x > 0) for x in lens]).cumsum(0)
+    again = cb.paged_prefill_attention(cache, q[last].contiguous().cuda(), starts.cuda(), 0.2).cpu()
+    for n, s in enumerate(last):
+        if s % 37 and lens[s] < 100:
+            continue
+        want, pv, size, js, p = R.attend(c, s, lens[s] - 1, q[s], 0.2)
+        tol = R.tolerance(want, pv, size, len(js), 32, F16, F16)
+        R.check(got[s], want, tol, f"sequence {s}")
+        R.check(again[n], want, tol, f"sequence {s} as a prompt")
+    assert not got[[i for i, x in enumerate(lens) if not x]].any()
+    assert float((w.sum(-1).cpu() - 2.0 * torch.tensor([[float(x > 0)] for x in lens])).abs().max()) < 1e-4
+    new = torch.randn(4096, 2, 32).half()
+    pos = torch.full((4096, 2, 208), -1, dtype=torch.int32).cuda()
+    cb.paged_append(cache, new.cuda(), new.cuda(), positions=pos)
+    kept, lens_out = cb.paged_evict(cache, w, torch.arange(208, dtype=torch.int32).expand(4096, 2, 208).contiguous().cuda(), 3, 1, 1)
+    assert torch.equal(lens_out.cpu(), torch.tensor([min(x, 3) for x in lens], dtype=torch.int32))
+    assert torch.equal((kept >= 0).sum(-1).cpu(), torch.tensor([[min(x, 3)] * 2 for x in lens]))
+    assert torch.equal((pos >= 0).sum(-1).cpu(), torch.tensor([[int(x > 0)] * 2 for x in lens]))
