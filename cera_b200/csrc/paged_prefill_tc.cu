@@ -38,6 +38,7 @@ namespace {
 
 constexpr uint32_t PP_ROWS = 128;
 constexpr float PP_LIFT = 7.0f, PP_RAISE = 8.0f;
+constexpr uint32_t PP_MATH_REGS = 208, PP_LOAD_REGS = 80;  // of a thread, where there are two tiles of rows: of 168 x 384 at the launch 1024 less
 constexpr uint32_t PP_MASKS = 4;  // tiles whose masks are kept: more than the keys' stages and one
 
 // Shapes by the padded head size and the number of parts.
@@ -723,10 +724,10 @@ __global__ void __launch_bounds__(Pp<DP, NP>::THREADS, 1) paged_prefill_tc_kerne
     const uint32_t tmem = tmem_at;
     unsigned int *status = &g_paged_prefill_status;
     if (warp < C::MATH) {
-        if (C::MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // of 168 x 384 at the launch: 208 x 256 + 80 x 128 are 1024 less
+        if (C::MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PP_MATH_REGS));
         pp_softmax<T, TQ, DP, NP>(p, w, warp / 4, qs, tmem, &bars, masks, &abort_s, status);
     } else {
-        if (C::MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (C::MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PP_LOAD_REGS));
         if (warp == C::MATH) {
             pp_multiply<T, DP, NP>(p, w, qs, ks, vs, tmem, &bars, &abort_s, status);
         } else if (warp < C::MATH + 3) {
@@ -754,6 +755,21 @@ uint32_t pp_tc_most(const PagedView &kv, size_t n_heads, size_t n) {
     return most;
 }
 
+// A warpgroup that asks for registers which the block was not launched with waits for good: a build that gave the kernel fewer is refused.
+template <auto KERNEL>
+int32_t pp_registers(uint32_t threads) {
+    static thread_local int asked = -1;
+    int dev = 0;
+    CERA_CUDA_TRY(cudaGetDevice(&dev));
+    if (asked == dev) return CERA_CUDA_OK;
+    cudaFuncAttributes a;
+    CERA_CUDA_TRY(cudaFuncGetAttributes(&a, KERNEL));
+    if ((uint32_t)(a.numRegs + 7) / 8 * 8 * threads < (threads - 128) * PP_MATH_REGS + 128 * PP_LOAD_REGS)
+        return fail(CERA_CUDA_ERR_UNSUPPORTED, "paged_prefill_attention: built with %d registers a thread", a.numRegs);
+    asked = dev;
+    return CERA_CUDA_OK;
+}
+
 template <typename T, typename TQ, int DP>
 int32_t pp_launch(PpParams &p, const PpGrid &g, int type, cudaStream_t st) {
     constexpr int NP = sizeof(TQ) == 2 ? 1 : std::is_same<T, __half>::value ? 2 : 3;
@@ -765,6 +781,7 @@ int32_t pp_launch(PpParams &p, const PpGrid &g, int type, cudaStream_t st) {
     if (!by_tma) p.box = C::KT;
     auto kernel = by_tma ? paged_prefill_tc_kernel<T, TQ, DP, NP, true> : paged_prefill_tc_kernel<T, TQ, DP, NP, false>;
     CERA_TRY((by_tma ? paged_smem<paged_prefill_tc_kernel<T, TQ, DP, NP, true>>(C::SMEM) : paged_smem<paged_prefill_tc_kernel<T, TQ, DP, NP, false>>(C::SMEM)));
+    if (C::MT == 2) CERA_TRY((by_tma ? pp_registers<paged_prefill_tc_kernel<T, TQ, DP, NP, true>>(C::THREADS) : pp_registers<paged_prefill_tc_kernel<T, TQ, DP, NP, false>>(C::THREADS)));
     count_launch();
     CERA_CUDA_TRY(launch_k(kernel, dim3(g.units, p.kv.hk, g.splits), dim3(C::THREADS), C::SMEM, st, mk, mv, p));
     return pp_join<T, TQ>(p, g, st);

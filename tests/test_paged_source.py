@@ -60,3 +60,13 @@ def test_loaders_wait_for_their_copies_before_they_leave():
         given_up = re.findall(r"if \(!tma::mbar_wait_warp\([^;]*?status, \d+u\)\) return drain\(", body)
         assert len(given_up) == waits == len(re.findall(r"mbar_wait_warp\(", text))
         assert re.fullmatch(r"drain\([^;]*\);\s*(return;\s*)?\}\s*(template <[^{]*)?", text[text.rindex("drain("):]), text[text.rindex("drain("):]
+
+
+def test_warpgroups_that_ask_for_registers_are_launched_with_enough():
+    """setmaxnreg.inc waits until the block has that many to spare, for good if it never had: the host asks before the launch, with the numbers that the kernel has."""
+    text = _text("paged_prefill_tc.cu")
+    assert re.findall(r'setmaxnreg\.(inc|dec)[^"]*%0;" ::"n"\((\w+)\)', text) == [("inc", "PP_MATH_REGS"), ("dec", "PP_LOAD_REGS")] and text.count("setmaxnreg") == 2
+    guard = text[text.index("int32_t pp_registers("):text.index("int32_t pp_launch(")]
+    assert "numRegs + 7) / 8 * 8 * threads < (threads - 128) * PP_MATH_REGS + 128 * PP_LOAD_REGS" in guard
+    launch = text[text.index("int32_t pp_launch("):]
+    assert launch.index("pp_registers<") < launch.index("launch_k(")
