@@ -242,7 +242,8 @@ int32_t cera_cuda_paged_evict(const cera_cuda_paged_kv *kv, const float *weights
     if (track_stride < cap || out_stride < (budget < cap ? budget : cap))
         return fail(CERA_CUDA_ERR_BAD_ARG, "%s: weights and positions of %zu slots into %zu (%zu, budget %zu)", what, track_stride, out_stride, cap, budget);
     if (v.n_seqs == 0) return CERA_CUDA_OK;
-    if (!weights_dev || !positions_dev || !weights_out_dev || !positions_out_dev || !kept_dev || !seq_lens_out_dev) return fail(CERA_CUDA_ERR_BAD_ARG, "%s: null argument", what);
+    if ((cap && (!weights_dev || !positions_dev || !weights_out_dev || !positions_out_dev)) || !kept_dev || !seq_lens_out_dev)  // of no slots there is nothing
+        return fail(CERA_CUDA_ERR_BAD_ARG, "%s: null argument", what);
     if ((weights_out_dev == weights_dev && out_stride != track_stride) || (positions_out_dev == positions_dev && out_stride != track_stride))
         return fail(CERA_CUDA_ERR_BAD_ARG, "%s: in place with another stride", what);
     return launch_paged_evict(v, kv->type, weights_dev, positions_dev, track_stride, budget, n_sink, n_recent, weights_out_dev, positions_out_dev, out_stride, kept_dev,

@@ -382,3 +382,25 @@ def test_as_many_sequences_as_there_may_be():
     assert torch.equal(lens_out.cpu(), torch.tensor([min(x, 3) for x in lens], dtype=torch.int32))
     assert torch.equal((kept >= 0).sum(-1).cpu(), torch.tensor([[min(x, 3)] * 2 for x in lens]))
     assert torch.equal((pos >= 0).sum(-1).cpu(), torch.tensor([[int(x > 0)] * 2 for x in lens]))
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_no_room_and_no_pages(types):
+    """Tables without columns, and caches without a page: nothing is seen, stored or kept that is not there."""
+    need_gpu()
+    import cera_b200 as cb
+    q, starts = _q(5, 4, 64, types[0]).cuda(), _i32([0, 2, 5])
+    new = _q(5, 2, 64, types[0]).cuda()
+    for pages, wide in ((4, 0), (0, 3), (0, 0)):
+        k, v = (torch.zeros(pages, 16, 2, 64, dtype=types[1], device="cuda") for _ in range(2))
+        lens = _i32([9, 40])
+        cache = cb.PagedKv(k, v, torch.zeros(2, wide, dtype=torch.int32, device="cuda"), lens)
+        cap = 16 * wide
+        w, p = torch.ones(2, 2, cap, device="cuda"), torch.arange(cap, dtype=torch.int32, device="cuda").expand(2, 2, cap).contiguous()
+        assert not cb.paged_decode_attention(cache, q[:2].contiguous(), 0.125).any()
+        assert not cb.paged_decode_attention(cache, q[:2].contiguous(), 0.125, weights=w, window=3, n_sink=1).any() and (w == 1).all()
+        assert not cb.paged_prefill_attention(cache, q, starts, 0.125).any()
+        cb.paged_append(cache, new, new, starts, weights=w, positions=p)
+        kept, lens_out = cb.paged_evict(cache, w, p, 4, 1, 1)
+        assert lens_out.tolist() == [min(x, cap, 4) for x in (9, 40)] and torch.equal((kept >= 0).sum(-1), lens_out[:, None].expand(2, 2).long())
+        assert not k.any() and not v.any()
