@@ -319,7 +319,7 @@ __device__ __forceinline__ void pp_multiply(const PpParams &p, const PpWork &w, 
 }
 
 // A tile's queries into shared memory -> the factor of the lane's row's scores, in units of ln 2.  f32: by warps, a row's pieces of 16 bytes a lane each (a thread a row, whose lines do
-// not stay in what shared memory leaves of L1, takes 37 us for a prompt of 512, this 32).  Others: a thread a row (8000 tokens through a window of 4096 in 473 us, by warps 487).
+// not stay in what shared memory leaves of L1, takes 37 us for a prompt of 512, this 32).  Others: a thread a row (8000 tokens through a window of 4096: by warps 3 % longer).
 template <typename T, typename TQ, int DP, int NP>
 __device__ __forceinline__ float pp_queries(const PpParams &p, const PpWork &w, uint32_t row, uint8_t *to, uint32_t r) {
     using C = Pp<DP, NP>;
@@ -479,7 +479,7 @@ __device__ __forceinline__ void pp_softmax(const PpParams &p, const PpWork &w, u
         }
         // f32 queries: weights for the maximum that is known; where the tile has a score past it by more than 2^8, O and the
         // sum are rescaled and the weights, whose scores are still in registers, formed again.  16-bit queries: the maximum first, then the weights' upper parts, which take
-        // the place of the scores, and the lower parts beside the upper ones' product (all of a weight at once: 752 us for 8000 tokens through a window of 4096, 615 so).
+        // the place of the scores, and the lower parts beside the upper ones' product (all of a weight at once: 752 us for 8000 tokens through a window of 4096, 620 so).
         constexpr int Q = C::KT / 32;
         uint32_t v[Q][32];
 #pragma unroll

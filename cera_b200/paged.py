@@ -183,7 +183,8 @@ def paged_evict(cache, weights, positions, budget, n_sink=0, n_recent=0, weights
     """Cuts every sequence and KV head down to `budget` slots -> (kept, seq_lens).  Kept are the slots with a position below n_sink or
     among the n_recent latest (newest position - n_recent < position), then those of the largest weight (a NaN is the smallest), ties
     to the lower slot.  What is kept past the budget moves, pages included, into the gaps below it, so slots lose their order: attend without
-    a window afterwards.  weights (float32) and positions (int32), [n_seqs, n_kv_heads, at least capacity], follow in place or into
+    a window afterwards.  Slots are picked whether their pages are there or not, and only rows that are there move: a cache that is evicted from should have
+    all its pages.  weights (float32) and positions (int32), [n_seqs, n_kv_heads, at least capacity], follow in place or into
     weights_out and positions_out (at least min(budget, capacity) slots).  kept, int32 [n_seqs, n_kv_heads, budget]: the slot that each slot's
     content came from, -1 past the length; seq_lens: min(length, budget) in a new tensor or in seq_lens_out, which may be
     cache.seq_lens.  Pages past the budget are the caller's again."""

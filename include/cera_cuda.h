@@ -215,7 +215,8 @@ CERA_API int32_t cera_cuda_decode_attention_noalloc(const float *q_dev, const vo
 /* [0, seq_lens[s]) are in use (a length outside [0, max_pages * page_size] counts */
 /* as the nearer end).  A table entry outside [0, n_pages) is a page that is not    */
 /* there: its slots are not seen, not stored to and not moved, so the pages that a   */
-/* window has left behind may be given back and their entries set to -1.            */
+/* window has left behind may be given back and their entries set to -1 (paged_evict picks slots without asking for their pages: a cache that is evicted  */
+/* from should have them all).                                                      */
 /* Sequences may share pages that are only read; what paged_append and paged_evict write must be in pages of one sequence.  head_dim: */
 /* a multiple of 32 up to 256; n_seqs up to 4096.  Nothing here synchronises; lengths  */
 /* and the table are read on the device, so a captured graph follows them.            */
